@@ -522,6 +522,134 @@ int rwkvmoe_ortho_backward(const rwkvmoe_desc* desc, const rwkvmoe_grads* g,
 int rwkvmoe_ortho_loss(const rwkvmoe_desc* desc, const rwkvmoe_tensors* t,
                        void* ws, size_t ws_bytes, void* stream);
 
+/* ---- routing to experts from logits ---------------------------------------- */
+
+enum rwkvmoe_score { RWKVMOE_SCORE_SOFTMAX = 0, RWKVMOE_SCORE_SIGMOID = 1 };
+enum rwkvmoe_group_score { RWKVMOE_GROUP_MAX = 0, RWKVMOE_GROUP_TOP2 = 1 };
+/* rwkvmoe_route_desc.flags: gates_i = scale · s_i / Σ_selected s (else scale · s_i) */
+#define RWKVMOE_ROUTE_RENORM 1
+
+typedef struct rwkvmoe_route_desc {
+  int32_t rows;          /* tokens (0: nothing is done) */
+  int32_t n_experts;     /* E, 1..512 */
+  int32_t top_k;         /* k, 1..min(32, top_groups · E / n_groups) */
+  int32_t n_groups;      /* G, 1..64, a divisor of E (1: no groups) */
+  int32_t top_groups;    /* 1..G */
+  int32_t dtype;         /* enum rwkvmoe_dtype of logits and d_logits */
+  int32_t score;         /* enum rwkvmoe_score */
+  int32_t group_score;   /* enum rwkvmoe_group_score */
+  int32_t flags;         /* RWKVMOE_ROUTE_RENORM */
+  float scale;
+  int64_t logits_stride; /* elements between the rows of logits, >= E */
+} rwkvmoe_route_desc;
+
+/* Experts and gates of every token from the router's logits (rows, E), with
+ * the options that models of many experts route by; the reference's Router
+ * (rwkv_mlx/moe.py:51-86) is the softmax case without groups and bias,
+ * renormalised.
+ *   s_e = softmax(l)_e or sigmoid(l_e)
+ *   experts are ranked by s_e + bias_e in 64 bits, or without a bias by l_e;
+ *   bias (E) fp32 or NULL only ranks, it is no part of a gate
+ *   n_groups > 1: consecutive groups of E / n_groups experts; only experts of
+ *   the best top_groups groups are ranked, a group counting as its best
+ *   expert's rank value (GROUP_MAX) or as the sum of s_e (+ bias_e) of its two
+ *   best (GROUP_TOP2)
+ *   inds (rows, k) int32, best first, ties to the lower index; gates (rows, k)
+ *   fp32 in the same order
+ * An expert whose logit is -inf or NaN, or whose bias is, takes no part: it
+ * comes after the others of the chosen groups (in index order) and its gate
+ * is 0.  A row with nothing left has valid, distinct inds and gates of 0. */
+int rwkvmoe_route(const rwkvmoe_route_desc* desc, const void* logits, const float* bias, int32_t* inds, float* gates,
+                  void* stream);
+
+/* VJP of rwkvmoe_route: d_logits (rows, E), dense, dtype, from d_gates
+ * (rows, k) fp32, with the forward's logits, inds and gates.  The selection is
+ * piecewise constant, and a slot whose gate is 0 has no gradient. */
+int rwkvmoe_route_backward(const rwkvmoe_route_desc* desc, const void* logits, const int32_t* inds, const float* gates,
+                           const float* d_gates, void* d_logits, void* stream);
+
+/* ---- 8-bit products with a scale for each block of 128 ---------------------- */
+
+/* A matrix (R, K) held in 8 bits is
+ *   q       (R, 128·Kb) e4m3 bytes (OCP, no infinities), Kb = ceil(K / 128),
+ *           zero from column K on
+ *   scales  fp32, (Kb, R) for blocks of 128 values of a row (FP8_ROWS), or
+ *           (ceil(R / 128), Kb) for blocks of 128 x 128 (FP8_TILES)
+ * and stands for q · scale.  Rounding a block with a = max(|v|, 2^-100):
+ * scale = fp32(a / 448), q = e4m3(v · fp32(448 / a)), to nearest even.  A NaN
+ * or an infinity makes its block NaN. */
+enum rwkvmoe_fp8_block { RWKVMOE_FP8_ROWS = 0, RWKVMOE_FP8_TILES = 1 };
+
+typedef struct rwkvmoe_fp8_desc {
+  int32_t rows;    /* rows of x and out, 0..8388480 */
+  int32_t n;       /* columns of out = rows of the weight (the products) */
+  int32_t k;       /* columns of x and of the weight, 1..8388608 */
+  int32_t groups;  /* 0: one matrix; else 1..1024 weights of the same shape */
+  int32_t dtype;   /* enum rwkvmoe_dtype of x and out */
+  int32_t block;   /* enum rwkvmoe_fp8_block (quantize: of the result; products: of b) */
+  int64_t stride;  /* elements between the rows of x, >= k (quantize, linear) */
+} rwkvmoe_fp8_desc;
+
+/* x (rows, k) in 8 bits: q, scales as above.  With q_t and scales_t also (or,
+ * with q NULL, only) the transpose (k, rows): FP8_ROWS rounds it in blocks of
+ * 128 values of a column of x, FP8_TILES transposes the blocks.  FP8_TILES
+ * takes `groups` matrices, one after the other. */
+int rwkvmoe_fp8_quantize(const rwkvmoe_fp8_desc* desc, const void* x, void* q, float* scales, void* q_t,
+                         float* scales_t, void* stream);
+
+/* A weight that is in 8 bits already, e4m3 (max(groups,1), n, k) unpadded with
+ * (.., ceil(n / 128), ceil(k / 128)) scales, laid out as above; with q_t and
+ * scales_t its transpose too (n and k of the desc are the source's). */
+int rwkvmoe_fp8_layout(const rwkvmoe_fp8_desc* desc, const void* src, const float* src_scales, void* q, float* scales,
+                       void* q_t, float* scales_t, void* stream);
+
+/* out (rows, n) = a · bᵀ, summed in fp32.  a is (rows, k) with FP8_ROWS
+ * scales; b (n, k) has FP8_TILES scales, or FP8_ROWS scales (groups 0).  With
+ * groups > 0 b holds that many weights, and row r is multiplied with weight g
+ * for offsets[g] <= r < offsets[g + 1] (offsets (groups + 1) ascending device
+ * int32, offsets[0] taken as 0, clamped to the rows); rows at or past
+ * offsets[groups] become 0. */
+int rwkvmoe_fp8_matmul(const rwkvmoe_fp8_desc* desc, const void* a, const float* a_scales, const void* b,
+                       const float* b_scales, const int32_t* offsets, void* out, void* stream);
+
+/* Scratch bytes of rwkvmoe_fp8_linear (host only). */
+int rwkvmoe_fp8_linear_workspace_bytes(const rwkvmoe_fp8_desc* desc, size_t* bytes);
+
+/* x (rows, k) rounded to FP8_ROWS and multiplied with b (FP8_TILES), as
+ * rwkvmoe_fp8_quantize and rwkvmoe_fp8_matmul do. */
+int rwkvmoe_fp8_linear(const rwkvmoe_fp8_desc* desc, const void* x, const void* b, const float* b_scales,
+                       const int32_t* offsets, void* out, void* ws, size_t ws_bytes, void* stream);
+
+/* Operands of rwkvmoe_fp8_experts_forward (device pointers). */
+typedef struct rwkvmoe_fp8_experts {
+  uint64_t struct_size;    /* sizeof(rwkvmoe_fp8_experts) */
+  const void* x;           /* (B,T,C), dtype */
+  const void* x_prev;      /* (B,C) with RWKVMOE_HAS_PREV, else NULL */
+  const void* x_k;         /* (E,C), dtype */
+  const void* key_q;       /* (E,F,C) in 8 bits, FP8_TILES */
+  const float* key_scales;
+  const void* value_q;     /* (E,C,F) in 8 bits, FP8_TILES */
+  const float* value_scales;
+  const int32_t* inds;     /* (N,k) experts; an id outside 0..E-1 is an unrouted slot */
+  const float* gates;      /* (N,k) fp32 */
+  const void* residual;    /* (B,T,C) with RWKVMOE_ADD_RESIDUAL, else NULL */
+  void* out;               /* (B,T,C), dtype */
+} rwkvmoe_fp8_experts;
+
+/* Scratch bytes of rwkvmoe_fp8_experts_forward (host only). */
+int rwkvmoe_fp8_experts_workspace_bytes(const rwkvmoe_desc* desc, size_t* bytes);
+
+/* The full-expert layer (moe.py:218-234) on a given routing, its two products
+ * in 8 bits:
+ *   xk = x + (shift(x) - x) · x_k[e]         fp32, rounded to FP8_ROWS
+ *   h  = relu(xk · keyᵀ)²                    fp32, rounded to FP8_ROWS
+ *   out[t] = Σ_slots gates · (h · valueᵀ)    fp32 (+ residual), one rounding
+ * Of desc: batch, seq_len, d_model (a multiple of 4), d_ffn, n_experts (1..64),
+ * top_k (1..8), dtype and the flags RWKVMOE_HAS_PREV and RWKVMOE_ADD_RESIDUAL.
+ * Only routed rows are computed; sums do not depend on timing. */
+int rwkvmoe_fp8_experts_forward(const rwkvmoe_desc* desc, const rwkvmoe_fp8_experts* t, void* ws, size_t ws_bytes,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,8 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "librwkvmoe.so"
 F32, F16, BF16 = 0, 1, 2
 MODE_FUSED, MODE_SPARSE = 0, 1
 HAS_PREV, HAS_BIAS, ADD_RESIDUAL = 1, 2, 4
+ROUTE_RENORM = 1
+FP8_ROWS, FP8_TILES = 0, 1
 GATE_F32, ADAPTERS_F32, GATES_F16, LORA_VALU, LN_IN = 8, 16, 32, 64, 128
 
 TORCH_DTYPE_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
@@ -55,6 +57,15 @@ ENTRY_POINTS = (
     "rwkvmoe_experts_forward",
     "rwkvmoe_experts_backward_workspace_bytes",
     "rwkvmoe_experts_backward",
+    "rwkvmoe_route",
+    "rwkvmoe_route_backward",
+    "rwkvmoe_fp8_quantize",
+    "rwkvmoe_fp8_layout",
+    "rwkvmoe_fp8_matmul",
+    "rwkvmoe_fp8_linear_workspace_bytes",
+    "rwkvmoe_fp8_linear",
+    "rwkvmoe_fp8_experts_workspace_bytes",
+    "rwkvmoe_fp8_experts_forward",
 )
 STAGE_ENTRY_POINTS = ("rwkvmoe_forward", "rwkvmoe_decode", "rwkvmoe_router_topk", "rwkvmoe_dispatch",
                       "rwkvmoe_cmix_key", "rwkvmoe_cmix_value", "rwkvmoe_lora_grouped", "rwkvmoe_combine",
@@ -107,6 +118,25 @@ class RouterGrads(ctypes.Structure):
 class LnGrads(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in (
         "x", "ln_weight", "d_y", "d_res", "d_x", "d_ln_weight", "d_ln_bias")]
+
+
+class RouteDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "rows", "n_experts", "top_k", "n_groups", "top_groups", "dtype", "score", "group_score", "flags")] + [
+        ("scale", ctypes.c_float), ("logits_stride", ctypes.c_int64)]
+
+
+class Fp8Desc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("rows", "n", "k", "groups", "dtype", "block")] + [
+        ("stride", ctypes.c_int64)]
+
+
+class Fp8Experts(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint64)] + [(n, ctypes.c_void_p) for n in (
+        "x", "x_prev", "x_k", "key_q", "key_scales", "value_q", "value_scales", "inds", "gates", "residual", "out")]
+
+
+FP8_EXPERTS_SIZE = ctypes.sizeof(Fp8Experts)
 
 
 class RwkvMoeError(RuntimeError):
@@ -176,6 +206,20 @@ def lib() -> ctypes.CDLL:
                                             ctypes.c_size_t, ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p),
                                             ctypes.c_int, ctypes.POINTER(ctypes.c_char_p),
                                             ctypes.POINTER(ctypes.c_int)]
+        vp, sz = ctypes.c_void_p, ctypes.c_size_t
+        for name, desc, args in (
+                ("rwkvmoe_route", RouteDesc, [vp] * 5),
+                ("rwkvmoe_route_backward", RouteDesc, [vp] * 6),
+                ("rwkvmoe_fp8_quantize", Fp8Desc, [vp] * 6),
+                ("rwkvmoe_fp8_layout", Fp8Desc, [vp] * 7),
+                ("rwkvmoe_fp8_matmul", Fp8Desc, [vp] * 7),
+                ("rwkvmoe_fp8_linear_workspace_bytes", Fp8Desc, [ctypes.POINTER(sz)]),
+                ("rwkvmoe_fp8_linear", Fp8Desc, [vp] * 6 + [sz, vp]),
+                ("rwkvmoe_fp8_experts_workspace_bytes", Desc, [ctypes.POINTER(sz)]),
+                ("rwkvmoe_fp8_experts_forward", Desc, [ctypes.POINTER(Fp8Experts), vp, sz, vp])):
+            f = getattr(h, name)
+            f.restype = ctypes.c_int
+            f.argtypes = [ctypes.POINTER(desc), *args]
         _LIB = h
     return _LIB
 
@@ -339,6 +383,53 @@ def experts_backward(desc: Desc, ws, ws_bytes: int, stream, **kw) -> None:
                                         stream)
     if st != 0:
         raise RwkvMoeError(st, "rwkvmoe_experts_backward")
+
+
+def check(status: int, where: str) -> None:
+    """Raise RwkvMoeError on a non-zero status."""
+    if status != 0:
+        raise RwkvMoeError(status, where)
+
+
+class _Here:
+    """The current device already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is current: a launch on a default stream
+    goes to the current device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+@lru_cache(maxsize=1024)
+def fp8_linear_bytes(rows, n, k, groups, dtype) -> int:
+    """Workspace of rwkvmoe_fp8_linear."""
+    desc = Fp8Desc(rows, n, k, groups, dtype, FP8_TILES, k)
+    b = ctypes.c_size_t(0)
+    check(lib().rwkvmoe_fp8_linear_workspace_bytes(ctypes.byref(desc), ctypes.byref(b)),
+          "rwkvmoe_fp8_linear_workspace_bytes")
+    return int(b.value)
+
+
+@lru_cache(maxsize=1024)
+def fp8_experts_plan(*dims) -> tuple[Desc, int]:
+    """The descriptor of rwkvmoe_fp8_experts_forward and its workspace."""
+    desc = Desc(*dims)
+    b = ctypes.c_size_t(0)
+    check(lib().rwkvmoe_fp8_experts_workspace_bytes(ctypes.byref(desc), ctypes.byref(b)),
+          "rwkvmoe_fp8_experts_workspace_bytes")
+    return desc, int(b.value)
 
 
 def ptr(t) -> int | None:

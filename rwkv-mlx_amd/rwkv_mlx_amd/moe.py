@@ -44,6 +44,7 @@ import torch
 from torch import nn
 
 from . import _lib
+from .fp8 import Fp8MoE_CMix
 from .model import _WS, RWKV_CMix_x070, RWKVConfig, operand, require_device
 
 __all__ = ["Router", "LoRAMoE_CMix", "MoE_CMix", "RWKV_CMix_x070", "RWKVConfig", "channel_mixing_rnn"]
@@ -855,6 +856,10 @@ def channel_mixing_rnn(x: torch.Tensor, x_prev: torch.Tensor, ffn: nn.Module, ln
     if isinstance(ffn, RWKV_CMix_x070):
         xs = x if ln is None else _ln_torch(x, *_ln_params(ln))
         out = ffn(xs.reshape(-1, 1, x.shape[-1]), x_prev=pb)
+        return out.reshape(x.shape), xs
+    if isinstance(ffn, Fp8MoE_CMix):
+        xs = x if ln is None else _ln_torch(x, *_ln_params(ln))
+        out = ffn(xs.reshape(-1, 1, x.shape[-1]), x_prev=pb)[0]
         return out.reshape(x.shape), xs
     raise TypeError(f"channel_mixing_rnn: unsupported ffn {type(ffn).__name__}")
 
