@@ -44,6 +44,15 @@ RWKV_DEV f32x4 mma128(i32x8 a, i32x8 b) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
 }
 
+// The same with the operands in accumulation registers and the result in
+// ordinary ones, which the fmas read: with more than 256 registers the compiler
+// itself would put the result the other way round and copy it.  The result is
+// there after 8 passes: two more of these have to be issued before it is read.
+RWKV_DEV void mma128_to(f32x4& d, i32x8 a, i32x8 b) {
+  asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, 0" : "=v"(d) : "a"(a), "a"(b));
+}
+RWKV_DEV void pin(f32x4& v) { asm volatile("" : "+v"(v)); }
+
 // The same in four steps of fp16: piece p is the p-th 8 bytes of a lane's 32.
 struct Wide {
   f16x8 p[4];
@@ -85,48 +94,6 @@ RWKV_DEV void load_lds4(__amdgpu_buffer_rsrc_t r, unsigned char* dst, unsigned v
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 4, voff, 0, 0, 0);
 }
 
-// The row range [lo, hi) of tile row mt and its group; group == p.groups: the
-// rows after the last range.  False: past every tile row.
-struct Range {
-  int lo, hi, g;
-};
-template <int BM>
-RWKV_DEV bool find_range(const Fp8Gemm& p, int mt, Range* r) {
-  const int lane = threadIdx.x & 63;
-  int before = 0, edge = 0;  // tiles and rows of the 64s of groups before
-  for (int g0 = 0; g0 <= p.groups; g0 += 64) {
-    const int g = g0 + lane;
-    // ranges are clamped to the rows, and do not overlap, whatever the offsets hold
-    int hi = g < p.groups ? min(max(p.off[g + 1], 0), p.m) : g == p.groups ? p.m : 0;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(hi, d);
-      if (lane >= d) hi = max(hi, v);
-    }
-    hi = max(hi, edge);
-    int lo = __shfl_up(hi, 1);
-    if (lane == 0) lo = edge;
-    edge = __builtin_amdgcn_readlane(hi, 63);
-    int sum = (hi - lo + BM - 1) / BM;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(sum, d);
-      if (lane >= d) sum += v;
-    }
-    const int found = __popcll(__ballot(before + sum <= mt));
-    if (found < 64) {
-      const int f = __builtin_amdgcn_readfirstlane(found);
-      const int prev = f > 0 ? __builtin_amdgcn_readlane(sum, f - 1) : 0;
-      r->g = g0 + f;
-      r->lo = __builtin_amdgcn_readlane(lo, f) + (mt - before - prev) * BM;
-      r->hi = __builtin_amdgcn_readlane(hi, f);
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(sum, 63);
-  }
-  return false;
-}
-
 template <typename T>
 RWKV_DEV void store4(T* row, int c, int n, bool vec, const float (&v)[4]) {
   if (vec && c + 4 <= n) {
@@ -148,174 +115,372 @@ template <> struct OutType<FP8_OUT_BF16> { typedef bf16 type; };
 
 // ---- tiles --------------------------------------------------------------------
 
-// A BM x BN tile, WGM x WGN waves.  Slices of one block of K (128 bytes a row)
-// go straight from memory into a ring of ST LDS stages; slice kb + ST - 1 is
-// requested as slice kb is multiplied, one barrier a slice.
-template <int BM, int BN, int WGM, int WGN, int ST, int BKIND, int OUT, bool GRP, bool EX>
-__global__ __launch_bounds__(WGM * WGN * 64) void fp8_tile_kernel(Fp8Gemm p, int tiles_m, int tiles_n, int group_m) {
+// The rows a tile row covers: [lo, hi) of group g (p.groups: the rows after the
+// last range, which become 0).
+struct Range {
+  int lo, hi, g;
+};
+
+// Tile rows of BM rows of every group, for the whole launch: lane l keeps group
+// l's range and the tile rows up to its end (up to 63 groups), else they are
+// summed again for every tile.  Ranges are clamped to the rows and do not
+// overlap, whatever the offsets hold.
+template <int BM> struct Ranges {
+  int lo, hi, sum, total;
+  bool kept;
+
+  // Groups g0 .. g0 + 63; edge: the row they start from.
+  static RWKV_DEV void scan(const Fp8Gemm& p, int g0, int edge, int* lo, int* hi, int* sum) {
+    const int lane = threadIdx.x & 63, g = g0 + lane;
+    int h = g < p.groups ? min(max(p.off[g + 1], 0), p.m) : g == p.groups ? p.m : 0;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(h, d);
+      if (lane >= d) h = max(h, v);
+    }
+    h = max(h, edge);
+    int l = __shfl_up(h, 1);
+    if (lane == 0) l = edge;
+    int n = (h - l + BM - 1) / BM;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(n, d);
+      if (lane >= d) n += v;
+    }
+    *lo = l;
+    *hi = h;
+    *sum = n;
+  }
+  RWKV_DEV void init(const Fp8Gemm& p) {
+    kept = p.groups < 64;
+    total = 0;
+    int edge = 0;
+    for (int g0 = 0; g0 <= p.groups; g0 += 64) {
+      scan(p, g0, edge, &lo, &hi, &sum);
+      edge = __builtin_amdgcn_readlane(hi, 63);
+      total += __builtin_amdgcn_readlane(sum, 63);
+    }
+  }
+  RWKV_DEV Range find(const Fp8Gemm& p, int mt) {
+    int g0 = 0, before = 0;
+    if (!kept) {
+      int edge = 0;
+      for (;; g0 += 64) {
+        scan(p, g0, edge, &lo, &hi, &sum);
+        const int n = __builtin_amdgcn_readlane(sum, 63);
+        if (mt < before + n) break;
+        before += n;
+        edge = __builtin_amdgcn_readlane(hi, 63);
+      }
+    }
+    const int f = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before + sum <= mt)));
+    const int prev = f > 0 ? __builtin_amdgcn_readlane(sum, f - 1) : 0;
+    return {__builtin_amdgcn_readlane(lo, f) + (mt - before - prev) * BM, __builtin_amdgcn_readlane(hi, f), g0 + f};
+  }
+};
+
+template <int N> struct Int { static constexpr int value = N; };
+
+// A BM x BN tile, WGM x WGN waves, one wave a SIMD: the registers of two hold
+// a bigger tile and the fragments ahead.  K is walked in slices of one block
+// (128 bytes a row), which go straight from memory into two LDS stages.
+//   * A slice is MI x NI steps: one MFMA, and the four fmas that scale the
+//     result of two steps before.  Rows of b (fragments j) stream through four
+//     registers sets, three ahead; the rows of a stay for the slice, and the
+//     next slice's are read into a second set.
+//   * One barrier a slice, three fragments of b before its end: every fragment
+//     of the slice has been read then, so its stage takes the requests of the
+//     slice after next, and the next slice has to have landed.
+//   * Workgroups are persistent and the slices run on across tiles.
+template <int BM, int BN, int WGM, int WGN, int PER_CU, int BKIND, int OUT, bool GRP, bool EX>
+__global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_tile_kernel(Fp8Gemm p, int tiles_m,
+                                                                                     int tiles_n, int group_m) {
   constexpr int NW = WGM * WGN;
   constexpr int WM = BM / WGM, WN = BN / WGN, MI = WM / 16, NI = WN / 16;
   constexpr int DA = BM / 8 / NW, DB = BN / 8 / NW;  // 1 KB requests of a wave a slice
   static_assert(DA * 8 * NW == BM && DB * 8 * NW == BN, "requests");
-  static_assert(BM / 64 + BN / 64 <= NW, "one scale request a wave");
+  constexpr int SA = BM / 64, SB = BKIND == FP8_ROWS ? BN / 64 : 0;
+  constexpr int DS = (SA + SB + NW - 1) / NW;        // 256 B requests of scales
+  constexpr int ND = DA + DB + DS;
   static_assert(128 % WN == 0 || WN == 128, "a wave's columns share one weight block");
   static_assert(OUT != FP8_OUT_RELU2Q || WN == 128, "a wave holds whole blocks of its rows");
-  constexpr int UA = BM * 128, UB = BN * 128, US = (BM + BN) * 4;
+  constexpr int UA = BM * 128, UB = BN * 128, US = NW * DS * 256;
   constexpr int STAGE = UA + UB + US;
-  static_assert(ST * STAGE <= 163840, "LDS");
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[ST * STAGE];
+  static_assert(PER_CU * 2 * STAGE <= 163840, "LDS");
+  constexpr bool ONE = NW * PER_CU == 4;             // one wave a SIMD
+  static_assert(!(ONE && EX), "the fp16 form is the compiler's");
+  constexpr int JB = NI - 3;                         // the barrier is in front of fragment JB of b
+  static_assert(NI % 4 == 0, "four fragments of b in turn");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WGN, wn = wave % WGN;
-  const int Kb = (p.k + 127) / 128, Kp = Kb * 128;
+  const int Kb = (p.k + 127) / 128, Kp = Kb * 128, Nb = (p.n + 127) / 128;
 
   // XCD w % 8 takes a contiguous run of the tiles, group_m tile rows at a time
-  const int total = tiles_m * tiles_n, w = blockIdx.x, xcd = w & 7;
-  const int l = xcd * (total / 8) + min(xcd, total % 8) + (w >> 3);
-  const int in_group = group_m * tiles_n, first = (l / in_group) * group_m;
-  const int gsize = min(tiles_m - first, group_m);
-  const int mt = first + (l % in_group) % gsize, n0 = ((l % in_group) / gsize) * BN;
-  Range r{mt * BM, p.m, 0};
+  Ranges<BM> ranges;
   if constexpr (GRP) {
-    if (!find_range<BM>(p, mt, &r)) return;
-    if (r.g == p.groups) {  // rows of no range
-      if constexpr (OUT != FP8_OUT_RELU2Q) {
-        typedef typename OutType<OUT>::type T;
-        for (int i = tid; i < BM * BN; i += NW * 64) {
-          const int row = r.lo + i / BN, c = n0 + i % BN;
-          if (row < r.hi && c < p.n) ((T*)p.out)[(size_t)row * p.n + c] = from_f<T>(0.f);
-        }
-      }
-      return;
-    }
+    ranges.init(p);
+    tiles_m = ranges.total;
   }
-  const int m0 = r.lo, mlim = min(r.hi, m0 + BM);
-
-  const __amdgpu_buffer_rsrc_t ra = buf_rsrc(p.a + (size_t)m0 * Kp, 0xFFFFFFF0u);
-  const __amdgpu_buffer_rsrc_t rb = buf_rsrc(p.b + ((size_t)r.g * p.n + n0) * Kp, 0xFFFFFFF0u);
-  unsigned va[DA], vb[DB];
-#pragma unroll
-  for (int i = 0; i < DA; ++i) {
-    const int row = (wave * DA + i) * 8 + (lane >> 3);
-    // rows past the end read the last one
-    va[i] = (unsigned)(min(m0 + row, mlim - 1) - m0) * (unsigned)Kp + ((lane & 7) ^ swz(row)) * 16;
-  }
-#pragma unroll
-  for (int i = 0; i < DB; ++i) {
-    const int row = (wave * DB + i) * 8 + (lane >> 3);
-    vb[i] = (unsigned)(min(n0 + row, p.n - 1) - n0) * (unsigned)Kp + ((lane & 7) ^ swz(row)) * 16;
-  }
-  // every wave makes one request of 64 scales: of a's rows, or of b's; with
-  // one scale a block of b the waves behind a's repeat them
-  const bool sb_wave = BKIND == FP8_ROWS && NW - 1 - wave < BN / 64;
-  const int sw = sb_wave ? NW - 1 - wave : wave % (BM / 64);
-  auto request = [&](int kb, int slot) {
-    unsigned char* st = lds + slot * STAGE;
-    const unsigned so = (unsigned)kb * 128u;
-#pragma unroll
-    for (int i = 0; i < DA; ++i)
-      load_lds16(ra, st + (wave * DA + i) * 1024, va[i], so);
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-      load_lds16(rb, st + UA + (wave * DB + i) * 1024, vb[i], so);
-    const float* sp = sb_wave ? p.sb + (size_t)kb * p.n + n0 : p.sa + (size_t)kb * p.m + m0;
-    const __amdgpu_buffer_rsrc_t rs = buf_rsrc(sp, (unsigned)(sb_wave ? min(BN, p.n - n0) : mlim - m0) * 4u);
-    load_lds4(rs, st + UA + UB + (sb_wave ? BM * 4 : 0) + sw * 256, (sw * 64 + lane) * 4);
+  const int total = tiles_m * tiles_n, G = gridDim.x, w = blockIdx.x, xcd = w & 7;
+  const int step = (G - xcd + 7) >> 3, run = total / 8 + (xcd < total % 8 ? 1 : 0);
+  const int base = xcd * (total / 8) + min(xcd, total % 8) + (w >> 3);
+  const int count = (w >> 3) < run ? (run - (w >> 3) + step - 1) / step : 0;
+  if (count == 0) return;
+  struct Tile {
+    int m0, mlim, n0, g;
+  };
+  auto tile_of = [&](int i) -> Tile {
+    const int l = base + i * step, in_group = group_m * tiles_n, first = (l / in_group) * group_m;
+    const int gsize = min(tiles_m - first, group_m), mt = first + (l % in_group) % gsize;
+    Range r{mt * BM, p.m, 0};
+    if constexpr (GRP) r = ranges.find(p, mt);
+    return {r.lo, min(r.hi, r.lo + BM), ((l % in_group) / gsize) * BN, r.g};
   };
 
-  // the weight block's scales along K
-  const int nb = (n0 + wn * WN) / 128;
-  const float* sbp = BKIND == FP8_TILES
-                         ? p.sb + ((size_t)r.g * ((p.n + 127) / 128) + min(nb, (p.n + 127) / 128 - 1)) * Kb
-                         : nullptr;
-  float sb_next = BKIND == FP8_TILES ? sbp[0] : 1.f;
+  // ---- requests: slice d_kb of tile d_i ----
+  __amdgpu_buffer_rsrc_t ra, rb;
+  unsigned va[DA], vb[DB];
+  const float* sbp = nullptr;  // the weight block's scales along K
+  int d_i = 0, d_kb = 0, d_m0 = 0, d_rows = 0, d_n0 = 0;
+  auto open_tile = [&]() {
+    const Tile t = tile_of(d_i);
+    int sl = lane;  // (opaque: addresses that depend on the lane alone would be kept in registers)
+    asm volatile("" : "+v"(sl));
+    const int g = GRP ? min(t.g, p.groups - 1) : 0;  // (tiles of no range multiply anything)
+    ra = buf_rsrc(p.a + (size_t)t.m0 * Kp, 0xFFFFFFF0u);
+    rb = buf_rsrc(p.b + ((size_t)g * p.n + t.n0) * Kp, 0xFFFFFFF0u);
+#pragma unroll
+    for (int i = 0; i < DA; ++i) {
+      const int row = (wave * DA + i) * 8 + (sl >> 3);
+      // rows past the end read the last one
+      va[i] = (unsigned)(min(t.m0 + row, t.mlim - 1) - t.m0) * (unsigned)Kp + ((sl & 7) ^ swz(row)) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < DB; ++i) {
+      const int row = (wave * DB + i) * 8 + (sl >> 3);
+      vb[i] = (unsigned)(min(t.n0 + row, p.n - 1) - t.n0) * (unsigned)Kp + ((sl & 7) ^ swz(row)) * 16;
+    }
+    if constexpr (BKIND == FP8_TILES)
+      sbp = p.sb + ((size_t)g * Nb + min((t.n0 + wn * WN) / 128, Nb - 1)) * Kb;
+    d_m0 = t.m0;
+    d_rows = t.mlim - t.m0;
+    d_n0 = t.n0;
+    d_kb = 0;
+  };
+  auto advance = [&]() {
+    if (d_kb + 1 < Kb) {
+      ++d_kb;
+    } else if (d_i + 1 < count) {
+      ++d_i;
+      open_tile();
+    }  // (past the last slice: it is requested again, into a stage that nothing reads any more)
+  };
+  auto request = [&](int stage, int q) {
+    unsigned char* st = lds + stage;
+    const unsigned so = (unsigned)d_kb * 128u;
+    if (q < DA) {
+      load_lds16(ra, st + (wave * DA + q) * 1024, va[q], so);
+    } else if (q < DA + DB) {
+      load_lds16(rb, st + UA + (wave * DB + q - DA) * 1024, vb[q - DA], so);
+    } else {
+      const int c = wave * DS + q - DA - DB;  // 64 scales: a's rows, then b's (further ones repeat)
+      const bool b = BKIND == FP8_ROWS && c >= SA;
+      const int c0 = b ? min(c - SA, SB - 1) : min(c, SA - 1);
+      const float* sp = b ? p.sb + (size_t)d_kb * p.n + d_n0 : p.sa + (size_t)d_kb * p.m + d_m0;
+      load_lds4(buf_rsrc(sp, (unsigned)(b ? min(BN, p.n - d_n0) : d_rows) * 4u), st + UA + UB + c * 256,
+                (c0 * 64 + lane) * 4);
+    }
+  };
 
+  // ---- fragments ----
   const int fsw = swz(lane & 15), fch = lane >> 4;
   const int ao = (wm * WM + (lane & 15)) * 128 + ((fch ^ fsw) << 4);
   const int bo = UA + (wn * WN + (lane & 15)) * 128 + ((fch ^ fsw) << 4);
-  f32x4 acc[MI][NI];
-#pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int so = UA + UB + (wm * WM + (lane & 15)) * 4;
+  const int co = UA + UB + SA * 256 + (wn * WN + (lane >> 4) * 4) * 4;
+  auto frag = [&](int at) { return join(*(const u32x4*)(lds + at), *(const u32x4*)(lds + (at ^ 64))); };
 
+  f32x4 acc[MI][NI];
+  auto zero_acc = [&]() {
 #pragma unroll
-  for (int s = 0; s < ST - 1; ++s) request(min(s, Kb - 1), s);
-  int slot = 0;
-  for (int kb = 0; kb < Kb; ++kb) {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * (DA + DB + 1)) : "memory");
-    const int free_slot = slot == 0 ? ST - 1 : slot - 1;
-    request(min(kb + ST - 1, Kb - 1), free_slot);  // (past the end: the last slice again, into a stage of no reader)
-    const float sb = sb_next;
-    if constexpr (BKIND == FP8_TILES) sb_next = sbp[min(kb + 1, Kb - 1)];
-    const unsigned char* st = lds + slot * STAGE;
-    typename Operand<EX>::type fa[MI];
-    float f[MI];
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      fa[i] = Operand<EX>::of(join(*(const u32x4*)(st + ao + i * 2048), *(const u32x4*)(st + (ao ^ 64) + i * 2048)));
-      f[i] = *(const float*)(st + UA + UB + (wm * WM + i * 16 + (lane & 15)) * 4) * sb;
-    }
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const auto fb =
-          Operand<EX>::of(join(*(const u32x4*)(st + bo + j * 2048), *(const u32x4*)(st + (bo ^ 64) + j * 2048)));
-      f32x4 cs{1.f, 1.f, 1.f, 1.f};
-      if constexpr (BKIND == FP8_ROWS)
-        cs = *(const f32x4*)(st + UA + UB + BM * 4 + (wn * WN + j * 16 + (lane >> 4) * 4) * 4);
+      for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  i32x8 fa[MI], ga[MI], fb[4];
+  f32x4 cs[BKIND == FP8_ROWS ? 4 : 1];
+  float f[MI], sa[MI];
+  float sb0 = 1.f, sb1 = 1.f;  // the weight's scale of this slice, and of the next
+
+  auto epilogue = [&](const Tile& it) {
+    int el = lane;
+    asm volatile("" : "+v"(el));
+    if constexpr (OUT == FP8_OUT_RELU2Q) {
+      const int col0 = it.n0 + wn * WN, Np = Nb * 128;
+      if (GRP && it.g == p.groups) return;
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        const f32x4 t = mma128(fb, fa[i]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          acc[i][j][q] = __builtin_fmaf(BKIND == FP8_ROWS ? t[q] * cs[q] : t[q], f[i], acc[i][j][q]);
-      }
-    }
-    slot = slot + 1 == ST ? 0 : slot + 1;
-  }
-
-  // ---- epilogue ----
-  if constexpr (OUT == FP8_OUT_RELU2Q) {
-    const int col0 = n0 + wn * WN;
-    const int Np = (p.n + 127) / 128 * 128;
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int row = m0 + wm * WM + i * 16 + (lane & 15);
-      unsigned am = 0;
-#pragma unroll
-      for (int j = 0; j < NI; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float v = acc[i][j][q], z = v < 0.f ? 0.f : v;  // (a NaN stays one)
-          acc[i][j][q] = col0 + j * 16 + (lane >> 4) * 4 + q < p.n ? z * z : 0.f;
-          am = umax(am, abs_bits(acc[i][j][q]));
-        }
-      am = umax(am, (unsigned)__shfl_xor((int)am, 16));
-      am = umax(am, (unsigned)__shfl_xor((int)am, 32));
-      const Fp8Factors fc = fp8_factors(am);
-      if (row < mlim && col0 < p.n) {
-        unsigned char* q = (unsigned char*)p.out + (size_t)row * Np + col0 + (lane >> 4) * 4;
+        const int row = it.m0 + wm * WM + i * 16 + (el & 15);
+        unsigned am = 0;
 #pragma unroll
         for (int j = 0; j < NI; ++j)
-          *(unsigned*)(q + j * 16) = fp8_pack4(acc[i][j][0] * fc.up, acc[i][j][1] * fc.up, acc[i][j][2] * fc.up,
-                                               acc[i][j][3] * fc.up);
-        if (lane < 16) p.out_s[(size_t)(col0 / 128) * p.m + row] = fc.down;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float v = acc[i][j][q], z = v < 0.f ? 0.f : v;  // (a NaN stays one)
+            acc[i][j][q] = col0 + j * 16 + (el >> 4) * 4 + q < p.n ? z * z : 0.f;
+            am = umax(am, abs_bits(acc[i][j][q]));
+          }
+        am = umax(am, (unsigned)__shfl_xor((int)am, 16));
+        am = umax(am, (unsigned)__shfl_xor((int)am, 32));
+        const Fp8Factors fc = fp8_factors(am);
+        if (row < it.mlim && col0 < p.n) {
+          unsigned char* q = (unsigned char*)p.out + (size_t)row * Np + col0 + (el >> 4) * 4;
+#pragma unroll
+          for (int j = 0; j < NI; ++j)
+            *(unsigned*)(q + j * 16) = fp8_pack4(acc[i][j][0] * fc.up, acc[i][j][1] * fc.up, acc[i][j][2] * fc.up,
+                                                 acc[i][j][3] * fc.up);
+          if (el < 16) p.out_s[(size_t)(col0 / 128) * p.m + row] = fc.down;
+        }
+      }
+    } else {
+      typedef typename OutType<OUT>::type T;
+      const bool none = GRP && it.g == p.groups, vec = p.n % 4 == 0;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int row = it.m0 + wm * WM + i * 16 + (el & 15);
+        if (row < it.mlim) {
+          T* o = (T*)p.out + (size_t)row * p.n;
+#pragma unroll
+          for (int j = 0; j < NI; ++j) {
+            float v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = none ? 0.f : acc[i][j][q];
+            store4<T>(o, it.n0 + wn * WN + j * 16 + (el >> 4) * 4, p.n, vec, v);
+          }
+        }
       }
     }
-  } else {
-    typedef typename OutType<OUT>::type T;
-    const bool vec = p.n % (8 / sizeof(T) * (sizeof(T) / 2)) == 0 && p.n % 4 == 0;
+  };
+
+  // One slice: stage `cur` (a byte offset), its a rows in xa; the next slice's
+  // (stage nxt) into ya.
+  auto slice = [&](i32x8 (&xa)[MI], i32x8 (&ya)[MI], int cur, int nxt) {
+    f32x4 t[3];
+    const float sbc = sb0;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int row = m0 + wm * WM + i * 16 + (lane & 15);
-      if (row >= mlim) continue;
-      T* o = (T*)p.out + (size_t)row * p.n;
+    for (int i = 0; i < MI; ++i) f[i] = sa[i] * sbc;
+    float sb2 = sb1;
+    f32x4 c0{1.f, 1.f, 1.f, 1.f}, c1 = c0;  // b's column scales of the step before, and of two before
+    auto scale = [&](int s, const f32x4& c) {
+      const int i = s % MI, j = s / MI;
+      pin(t[s % 3]);  // (neither before this point, nor later than it)
+      const f32x4 v = t[s % 3];
 #pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        store4<T>(o, n0 + wn * WN + j * 16 + (lane >> 4) * 4, p.n, vec, v);
+      for (int q = 0; q < 4; ++q)
+        acc[i][j][q] = __builtin_fmaf(BKIND == FP8_ROWS ? v[q] * c[q] : v[q], f[i], acc[i][j][q]);
+      pin(acc[i][j]);
+    };
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      if (j == JB) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        advance();
+        if constexpr (BKIND == FP8_TILES) sb2 = sbp[d_kb];
       }
+      auto wb = Operand<EX>::of(fb[j & 3]);
+      const f32x4 cj = BKIND == FP8_ROWS ? cs[j & 3] : c0;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int s = j * MI + i;
+        if constexpr (ONE) mma128_to(t[s % 3], wb, xa[i]);
+        else t[s % 3] = mma128(wb, Operand<EX>::of(xa[i]));
+        __builtin_amdgcn_sched_barrier(0);
+        if (s >= 2) scale(s - 2, c1);
+        c1 = c0;
+        c0 = cj;
+        if (i == 0) {  // fragment j + 3 of b, from NI on the next slice's
+          const int e = j + 3;
+          fb[e & 3] = frag((e < NI ? cur : nxt) + bo + (e % NI) * 2048);
+          if constexpr (BKIND == FP8_ROWS)
+            cs[e & 3] = *(const f32x4*)(lds + (e < NI ? cur : nxt) + co + (e % NI) * 64);
+        }
+        if (j >= JB) {
+          const int u = s - JB * MI;  // of 3 · MI
+          if (u % 3 == 1) {
+            ya[u / 3] = frag(nxt + ao + (u / 3) * 2048);
+            sa[u / 3] = *(const float*)(lds + nxt + so + (u / 3) * 64);
+          }
+#pragma unroll
+          for (int q = 0; q < ND; ++q)
+            if (q * 3 * MI / ND == u) request(cur, q);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (ONE) {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_nop 15" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    scale(NI * MI - 2, c1);
+    scale(NI * MI - 1, c0);
+    sb0 = sb1;
+    sb1 = sb2;
+  };
+
+  // ---- the first two slices ----
+  open_tile();
+  if constexpr (BKIND == FP8_TILES) sb0 = sbp[0];
+#pragma unroll
+  for (int q = 0; q < ND; ++q) request(0, q);
+  advance();
+  if constexpr (BKIND == FP8_TILES) sb1 = sbp[d_kb];
+#pragma unroll
+  for (int q = 0; q < ND; ++q) request(STAGE, q);
+  zero_acc();
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(ND) : "memory");
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    fa[i] = frag(ao + i * 2048);
+    sa[i] = *(const float*)(lds + so + i * 64);
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    fb[j] = frag(bo + j * 2048);
+    if constexpr (BKIND == FP8_ROWS) cs[j] = *(const f32x4*)(lds + co + j * 64);
+  }
+
+  if constexpr (ONE) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) asm volatile("" : "+a"(fa[i]));
+#pragma unroll
+    for (int j = 0; j < 3; ++j) asm volatile("" : "+a"(fb[j]));
+  }
+  int ci = 0, kb = 0;
+  // true after the last slice of the last tile
+  auto next = [&]() {
+    if (++kb < Kb) return false;
+    epilogue(tile_of(ci));
+    if (++ci == count) return true;
+    zero_acc();
+    kb = 0;
+    return false;
+  };
+  for (;;) {
+    slice(fa, ga, 0, STAGE);
+    if (next()) break;
+    slice(ga, fa, STAGE, 0);
+    if (next()) break;
+    if constexpr (ONE) {  // whole registers go round the loop (halves would be put together again)
+#pragma unroll
+      for (int i = 0; i < MI; ++i) asm volatile("" : "+a"(fa[i]));
+#pragma unroll
+      for (int j = 0; j < 3; ++j) asm volatile("" : "+a"(fb[j]));
     }
   }
   // requests into LDS land before the workgroup ends
@@ -428,12 +593,13 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Gemm p) {
   }
 }
 
-template <int BM, int BN, int WGM, int WGN, int ST, int BKIND, int OUT, bool GRP, bool EX>
+template <int BM, int BN, int WGM, int WGN, int PER_CU, int BKIND, int OUT, bool GRP, bool EX>
 hipError_t run_tile(const Fp8Gemm& p, hipStream_t s) {
   const int tiles_n = (p.n + BN - 1) / BN;
   const int tiles_m = (p.m + BM - 1) / BM + (GRP ? p.groups : 0);
-  launch_kernel((fp8_tile_kernel<BM, BN, WGM, WGN, ST, BKIND, OUT, GRP, EX>), dim3(tiles_m * tiles_n),
-                dim3(WGM * WGN * 64), 0, s, p, tiles_m, tiles_n, walk_group_m(tiles_m, tiles_n, BM, BN));
+  launch_kernel((fp8_tile_kernel<BM, BN, WGM, WGN, PER_CU, BKIND, OUT, GRP, EX>),
+                dim3(std::min(tiles_m * tiles_n, num_cus() * PER_CU)), dim3(WGM * WGN * 64), 0, s, p, tiles_m, tiles_n,
+                walk_group_m(tiles_m, tiles_n, BM, BN));
   return hipGetLastError();
 }
 
@@ -446,8 +612,10 @@ hipError_t run_few(const Fp8Gemm& p, hipStream_t s) {
 
 template <int BKIND, int OUT, bool GRP, bool EX>
 hipError_t run_tiles(const Fp8Gemm& p, hipStream_t s) {
-  const long long big = (long long)((p.m + 255) / 256) * ((p.n + 255) / 256);
-  if (big >= num_cus() * 3 / 4) return run_tile<256, 256, 4, 2, 2, BKIND, OUT, GRP, EX>(p, s);
+  if constexpr (!EX && BKIND == FP8_TILES) {
+    const long long big = (long long)((p.m + 191) / 192) * ((p.n + 255) / 256);
+    if (big >= num_cus() * 3 / 4) return run_tile<192, 256, 2, 2, 1, BKIND, OUT, GRP, EX>(p, s);
+  }
   return run_tile<128, 128, 4, 1, 2, BKIND, OUT, GRP, EX>(p, s);
 }
 
