@@ -183,7 +183,7 @@ template <int N> struct Int { static constexpr int value = N; };
 
 // A BM x BN tile, WGM x WGN waves, one wave a SIMD: the registers of two hold
 // a bigger tile and the fragments ahead.  K is walked in slices of one block
-// (128 bytes a row), which go straight from memory into two LDS stages.
+// (128 bytes a row), which go straight from memory into LDS rings.
 //   * A slice is MI x NI steps: one MFMA, and the four fmas that scale the
 //     result of two steps before.  Rows of b (fragments j) stream through four
 //     registers sets, three ahead; the rows of a stay for the slice, and the
@@ -192,26 +192,29 @@ template <int N> struct Int { static constexpr int value = N; };
 //     of the slice has been read then, so its stage takes the requests of the
 //     slice after next, and the next slice has to have landed.
 //   * Workgroups are persistent and the slices run on across tiles.
-template <int BM, int BN, int WGM, int WGN, int PER_CU, int BKIND, int OUT, bool GRP, bool EX>
+template <int BM, int BN, int WGM, int WGN, int PER_CU, int NB, int BKIND, int OUT, bool GRP, bool EX>
 __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_tile_kernel(Fp8Gemm p, int tiles_m,
                                                                                      int tiles_n, int group_m) {
   constexpr int NW = WGM * WGN;
   constexpr int WM = BM / WGM, WN = BN / WGN, MI = WM / 16, NI = WN / 16;
   constexpr int DA = BM / 8 / NW, DB = BN / 8 / NW;  // 1 KB requests of a wave a slice
   static_assert(DA * 8 * NW == BM && DB * 8 * NW == BN, "requests");
-  constexpr int SA = BM / 64, SB = BKIND == FP8_ROWS ? BN / 64 : 0;
-  constexpr int DS = (SA + SB + NW - 1) / NW;        // 256 B requests of scales
-  constexpr int ND = DA + DB + DS;
+  // 256 B requests of scales: with a its rows' and the weight blocks', with b its columns'
+  constexpr bool ROWS = BKIND == FP8_ROWS;
+  constexpr int SA = BM / 64, SB = BN / 64;
+  static_assert(SA + 1 <= NW && SB <= NW, "one request of scales a wave");
+  constexpr int DAS = DA + 1, DBS = DB + (ROWS ? 1 : 0);
   static_assert(128 % WN == 0 || WN == 128, "a wave's columns share one weight block");
   static_assert(OUT != FP8_OUT_RELU2Q || WN == 128, "a wave holds whole blocks of its rows");
-  constexpr int UA = BM * 128, UB = BN * 128, US = NW * DS * 256;
-  constexpr int STAGE = UA + UB + US;
-  static_assert(PER_CU * 2 * STAGE <= 163840, "LDS");
+  constexpr int UA = BM * 128, UB = BN * 128 + (ROWS ? NW * 256 : 0), US = NW * 256;
+  constexpr int STA = UA + US, B0 = 2 * STA;         // a's stages, then b's
+  constexpr int LDS_BYTES = B0 + NB * UB;
+  static_assert(PER_CU * LDS_BYTES <= 163840, "LDS");
   constexpr bool ONE = NW * PER_CU == 4;             // one wave a SIMD
   static_assert(!(ONE && EX), "the fp16 form is the compiler's");
   constexpr int JB = NI - 3;                         // the barrier is in front of fragment JB of b
   static_assert(NI % 4 == 0, "four fragments of b in turn");
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[LDS_BYTES];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -232,7 +235,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
   struct Tile {
     int m0, mlim, n0, g;
   };
-  auto tile_of = [&](int i) -> Tile {
+  auto tile_of = [&](int i) __attribute__((always_inline)) -> Tile {
     const int l = base + i * step, in_group = group_m * tiles_n, first = (l / in_group) * group_m;
     const int gsize = min(tiles_m - first, group_m), mt = first + (l % in_group) % gsize;
     Range r{mt * BM, p.m, 0};
@@ -240,71 +243,94 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
     return {r.lo, min(r.hi, r.lo + BM), ((l % in_group) / gsize) * BN, r.g};
   };
 
-  // ---- requests: slice d_kb of tile d_i ----
+  // ---- requests: slice kb of tile i of a (with the scales), and of b further on ----
+  struct Ahead {
+    int i, kb;
+  };
+  Ahead da{0, 0}, db{0, 0};
   __amdgpu_buffer_rsrc_t ra, rb;
   unsigned va[DA], vb[DB];
-  const float* sbp = nullptr;  // the weight block's scales along K
-  int d_i = 0, d_kb = 0, d_m0 = 0, d_rows = 0, d_n0 = 0;
-  auto open_tile = [&]() {
-    const Tile t = tile_of(d_i);
+  const float* sbp = nullptr;  // the scales of b: of a tile's weight blocks, or columns
+  int a_m0 = 0, a_rows = 0, b_scales = 0;
+  auto open_a = [&]() __attribute__((always_inline)) {
+    const Tile t = tile_of(da.i);
     int sl = lane;  // (opaque: addresses that depend on the lane alone would be kept in registers)
     asm volatile("" : "+v"(sl));
-    const int g = GRP ? min(t.g, p.groups - 1) : 0;  // (tiles of no range multiply anything)
     ra = buf_rsrc(p.a + (size_t)t.m0 * Kp, 0xFFFFFFF0u);
-    rb = buf_rsrc(p.b + ((size_t)g * p.n + t.n0) * Kp, 0xFFFFFFF0u);
 #pragma unroll
     for (int i = 0; i < DA; ++i) {
       const int row = (wave * DA + i) * 8 + (sl >> 3);
       // rows past the end read the last one
       va[i] = (unsigned)(min(t.m0 + row, t.mlim - 1) - t.m0) * (unsigned)Kp + ((sl & 7) ^ swz(row)) * 16;
     }
+    a_m0 = t.m0;
+    a_rows = t.mlim - t.m0;
+    if constexpr (!ROWS) {
+      sbp = p.sb + ((size_t)(GRP ? min(t.g, p.groups - 1) : 0) * Nb + t.n0 / 128) * Kb;
+      b_scales = min(BN / 128, Nb - t.n0 / 128) * Kb;
+    }
+  };
+  auto open_b = [&]() __attribute__((always_inline)) {
+    const Tile t = tile_of(db.i);
+    int sl = lane;
+    asm volatile("" : "+v"(sl));
+    const int g = GRP ? min(t.g, p.groups - 1) : 0;  // (tiles of no range multiply anything)
+    rb = buf_rsrc(p.b + ((size_t)g * p.n + t.n0) * Kp, 0xFFFFFFF0u);
 #pragma unroll
     for (int i = 0; i < DB; ++i) {
       const int row = (wave * DB + i) * 8 + (sl >> 3);
       vb[i] = (unsigned)(min(t.n0 + row, p.n - 1) - t.n0) * (unsigned)Kp + ((sl & 7) ^ swz(row)) * 16;
     }
-    if constexpr (BKIND == FP8_TILES)
-      sbp = p.sb + ((size_t)g * Nb + min((t.n0 + wn * WN) / 128, Nb - 1)) * Kb;
-    d_m0 = t.m0;
-    d_rows = t.mlim - t.m0;
-    d_n0 = t.n0;
-    d_kb = 0;
+    if constexpr (ROWS) {
+      sbp = p.sb + t.n0;
+      b_scales = min(BN, p.n - t.n0);
+    }
   };
-  auto advance = [&]() {
-    if (d_kb + 1 < Kb) {
-      ++d_kb;
-    } else if (d_i + 1 < count) {
-      ++d_i;
-      open_tile();
-    }  // (past the last slice: it is requested again, into a stage that nothing reads any more)
+  // (past the last slice it is requested again, into a stage that nothing reads any more)
+  auto advance = [&](Ahead& d, auto open) __attribute__((always_inline)) {
+    if (d.kb + 1 < Kb) {
+      ++d.kb;
+    } else if (d.i + 1 < count) {
+      ++d.i;
+      d.kb = 0;
+      open();
+    }
   };
-  auto request = [&](int stage, int q) {
+  auto request_a = [&](int stage, int q) __attribute__((always_inline)) {
     unsigned char* st = lds + stage;
-    const unsigned so = (unsigned)d_kb * 128u;
     if (q < DA) {
-      load_lds16(ra, st + (wave * DA + q) * 1024, va[q], so);
-    } else if (q < DA + DB) {
-      load_lds16(rb, st + UA + (wave * DB + q - DA) * 1024, vb[q - DA], so);
+      load_lds16(ra, st + (wave * DA + q) * 1024, va[q], (unsigned)da.kb * 128u);
+    } else {  // wave w: 64 rows' scales, or the weight blocks'; further waves repeat those
+      const bool b = !ROWS && wave >= SA;
+      const int c = min(wave, SA - 1), at = b ? (lane & 1) * Kb + da.kb : c * 64 + lane;
+      load_lds4(buf_rsrc(b ? sbp : p.sa + (size_t)da.kb * p.m + a_m0, (unsigned)(b ? b_scales : a_rows) * 4u),
+                st + UA + wave * 256, at * 4);
+    }
+  };
+  auto request_b = [&](int stage, int q) __attribute__((always_inline)) {
+    unsigned char* st = lds + stage;
+    if (q < DB) {
+      load_lds16(rb, st + (wave * DB + q) * 1024, vb[q], (unsigned)db.kb * 128u);
     } else {
-      const int c = wave * DS + q - DA - DB;  // 64 scales: a's rows, then b's (further ones repeat)
-      const bool b = BKIND == FP8_ROWS && c >= SA;
-      const int c0 = b ? min(c - SA, SB - 1) : min(c, SA - 1);
-      const float* sp = b ? p.sb + (size_t)d_kb * p.n + d_n0 : p.sa + (size_t)d_kb * p.m + d_m0;
-      load_lds4(buf_rsrc(sp, (unsigned)(b ? min(BN, p.n - d_n0) : d_rows) * 4u), st + UA + UB + c * 256,
-                (c0 * 64 + lane) * 4);
+      const int c = min(wave, SB - 1);
+      load_lds4(buf_rsrc(sbp + (size_t)db.kb * p.n, (unsigned)b_scales * 4u), st + BN * 128 + wave * 256,
+                (c * 64 + lane) * 4);
     }
   };
 
   // ---- fragments ----
   const int fsw = swz(lane & 15), fch = lane >> 4;
   const int ao = (wm * WM + (lane & 15)) * 128 + ((fch ^ fsw) << 4);
-  const int bo = UA + (wn * WN + (lane & 15)) * 128 + ((fch ^ fsw) << 4);
-  const int so = UA + UB + (wm * WM + (lane & 15)) * 4;
-  const int co = UA + UB + SA * 256 + (wn * WN + (lane >> 4) * 4) * 4;
-  auto frag = [&](int at) { return join(*(const u32x4*)(lds + at), *(const u32x4*)(lds + (at ^ 64))); };
+  const int bo = B0 + (wn * WN + (lane & 15)) * 128 + ((fch ^ fsw) << 4);
+  const int so = UA + (wm * WM + (lane & 15)) * 4;
+  // b's scales of this wave's columns: by column, or one for all
+  const int co = ROWS ? B0 + BN * 128 + (wn * WN + (lane >> 4) * 4) * 4 : UA + SA * 256 + wn * WN / 128 * 4;
+  auto frag = [&](int at) __attribute__((always_inline)) {
+    return join(*(const u32x4*)(lds + at), *(const u32x4*)(lds + (at ^ 64)));
+  };
 
   f32x4 acc[MI][NI];
-  auto zero_acc = [&]() {
+  auto zero_acc = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -312,10 +338,15 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
   };
   i32x8 fa[MI], ga[MI], fb[4];
   f32x4 cs[BKIND == FP8_ROWS ? 4 : 1];
-  float f[MI], sa[MI];
-  float sb0 = 1.f, sb1 = 1.f;  // the weight's scale of this slice, and of the next
+  float f[MI], sa[MI], sb = 1.f;
 
-  auto epilogue = [&](const Tile& it) {
+  // stores of whole 16 bytes, NST of them a tile, which may be in flight through the next tile's first slice
+  constexpr int NST = MI * NI * (OUT == FP8_OUT_F32 ? 2 : 1) / 2;
+  constexpr int WV = DAS + (NB - 2) * DBS;  // requests behind the slice that has to have landed
+  static_assert(WV + NST < 64, "vmcnt range");
+  const bool whole = OUT == FP8_OUT_RELU2Q || p.n % (OUT == FP8_OUT_F32 ? 4 : 8) == 0;
+  bool stores = false;
+  auto epilogue = [&](const Tile& it) __attribute__((always_inline)) {
     int el = lane;
     asm volatile("" : "+v"(el));
     if constexpr (OUT == FP8_OUT_RELU2Q) {
@@ -347,34 +378,75 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
       }
     } else {
       typedef typename OutType<OUT>::type T;
-      const bool none = GRP && it.g == p.groups, vec = p.n % 4 == 0;
+      const bool none = GRP && it.g == p.groups;
+      const int rows = it.mlim - it.m0, col0 = it.n0 + wn * WN;
+      if (whole) {
+        // 16 bytes a lane.  16-bit results: of two blocks of 16 columns, exchanged between the 16-lane rows so that
+        // lanes 0-15 and 32-47 hold the first one's two halves, the others the second one's; a store covers 64
+        // consecutive bytes of 16 rows.  Offsets past the rows or columns are dropped by the buffer's bound.
+        const __amdgpu_buffer_rsrc_t ro =
+            buf_rsrc((T*)p.out + (size_t)it.m0 * p.n, (unsigned)rows * (unsigned)p.n * (unsigned)sizeof(T));
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int row = it.m0 + wm * WM + i * 16 + (el & 15);
-        if (row < it.mlim) {
-          T* o = (T*)p.out + (size_t)row * p.n;
+        for (int i = 0; i < MI; ++i) {
+          const int row = wm * WM + i * 16 + (el & 15);
+          if constexpr (sizeof(T) == 2) {
 #pragma unroll
-          for (int j = 0; j < NI; ++j) {
-            float v[4];
+            for (int j = 0; j < NI; j += 2) {
+              unsigned v[2][2];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = none ? 0.f : acc[i][j][q];
-            store4<T>(o, it.n0 + wn * WN + j * 16 + (el >> 4) * 4, p.n, vec, v);
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  union { T e[2]; unsigned u; } w;
+                  w.e[0] = from_f<T>(none ? 0.f : acc[i][j + h][q * 2]);
+                  w.e[1] = from_f<T>(none ? 0.f : acc[i][j + h][q * 2 + 1]);
+                  v[h][q] = w.u;
+                }
+              const auto x = __builtin_amdgcn_permlane16_swap(v[0][0], v[1][0], false, false);
+              const auto y = __builtin_amdgcn_permlane16_swap(v[0][1], v[1][1], false, false);
+              const int c = col0 + (j + ((el >> 4) & 1)) * 16 + (el >> 5) * 8;
+              const unsigned off = c < p.n ? ((unsigned)row * (unsigned)p.n + c) * 2u : kOOB;
+              __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], y[0], x[1], y[1]}, ro, off, 0, 0);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+              const int c = col0 + j * 16 + (el >> 4) * 4;
+              const unsigned off = c < p.n ? ((unsigned)row * (unsigned)p.n + c) * 4u : kOOB;
+              f32x4 v = acc[i][j];
+              if (none) v = f32x4{0.f, 0.f, 0.f, 0.f};
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), ro, off, 0, 0);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          const int row = wm * WM + i * 16 + (el & 15);
+          if (row < rows) {
+            T* o = (T*)p.out + (size_t)(it.m0 + row) * p.n;
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int c = col0 + j * 16 + (el >> 4) * 4 + q;
+                if (c < p.n) o[c] = from_f<T>(none ? 0.f : acc[i][j][q]);
+              }
           }
         }
       }
     }
   };
 
-  // One slice: stage `cur` (a byte offset), its a rows in xa; the next slice's
-  // (stage nxt) into ya.
-  auto slice = [&](i32x8 (&xa)[MI], i32x8 (&ya)[MI], int cur, int nxt) {
+  // One slice: a's rows in xa, its stage `cur`; the next slice's (stage nxt)
+  // into ya.  b_cur, b_nxt: b's stages.
+  int b_cur = 0, b_nxt = NB > 1 ? UB : 0;
+  auto slice = [&](i32x8 (&xa)[MI], i32x8 (&ya)[MI], int cur, int nxt) __attribute__((always_inline)) {
     f32x4 t[3];
-    const float sbc = sb0;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) f[i] = sa[i] * sbc;
-    float sb2 = sb1;
+    for (int i = 0; i < MI; ++i) f[i] = sa[i] * sb;
     f32x4 c0{1.f, 1.f, 1.f, 1.f}, c1 = c0;  // b's column scales of the step before, and of two before
-    auto scale = [&](int s, const f32x4& c) {
+    auto scale = [&](int s, const f32x4& c) __attribute__((always_inline)) {
       const int i = s % MI, j = s / MI;
       pin(t[s % 3]);  // (neither before this point, nor later than it)
       const f32x4 v = t[s % 3];
@@ -383,15 +455,9 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
         acc[i][j][q] = __builtin_fmaf(BKIND == FP8_ROWS ? v[q] * c[q] : v[q], f[i], acc[i][j][q]);
       pin(acc[i][j]);
     };
+    auto steps = [&](auto from, auto to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      if (j == JB) {
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        advance();
-        if constexpr (BKIND == FP8_TILES) sb2 = sbp[d_kb];
-      }
+    for (int j = decltype(from)::value; j < decltype(to)::value; ++j) {
       auto wb = Operand<EX>::of(fb[j & 3]);
       const f32x4 cj = BKIND == FP8_ROWS ? cs[j & 3] : c0;
 #pragma unroll
@@ -405,23 +471,47 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
         c0 = cj;
         if (i == 0) {  // fragment j + 3 of b, from NI on the next slice's
           const int e = j + 3;
-          fb[e & 3] = frag((e < NI ? cur : nxt) + bo + (e % NI) * 2048);
+          fb[e & 3] = frag((e < NI ? b_cur : b_nxt) + bo + (e % NI) * 2048);
           if constexpr (BKIND == FP8_ROWS)
-            cs[e & 3] = *(const f32x4*)(lds + (e < NI ? cur : nxt) + co + (e % NI) * 64);
+            cs[e & 3] = *(const f32x4*)(lds + (e < NI ? b_cur : b_nxt) + co + (e % NI) * 64);
+        }
+        if (j >= 1 && j < JB) {
+          constexpr int U = (JB - 1) * MI;
+#pragma unroll
+          for (int q = 0; q < DAS; ++q)
+            if (q * U / DAS == s - MI) request_a(cur, q);
         }
         if (j >= JB) {
           const int u = s - JB * MI;  // of 3 · MI
           if (u % 3 == 1) {
             ya[u / 3] = frag(nxt + ao + (u / 3) * 2048);
             sa[u / 3] = *(const float*)(lds + nxt + so + (u / 3) * 64);
+            if (BKIND == FP8_TILES && u == 1) sb = *(const float*)(lds + nxt + co);
           }
 #pragma unroll
-          for (int q = 0; q < ND; ++q)
-            if (q * 3 * MI / ND == u) request(cur, q);
+          for (int q = 0; q < DBS; ++q)
+            if (q * 3 * MI / DBS == u) request_b(B0 + b_cur, q);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    };
+    steps(Int<0>{}, Int<1>{});
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    advance(da, open_a);
+    steps(Int<1>{}, Int<JB>{});
+    __builtin_amdgcn_sched_barrier(0);
+    if (stores && OUT != FP8_OUT_RELU2Q) {  // (behind them: this slice's requests of a)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WV + NST) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WV) : "memory");
+    }
+    stores = false;
+    __builtin_amdgcn_sched_barrier(0);
+    advance(db, open_b);
+    steps(Int<JB>{}, Int<NI>{});
     if constexpr (ONE) {
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("s_nop 15" ::: "memory");
@@ -429,26 +519,32 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
     }
     scale(NI * MI - 2, c1);
     scale(NI * MI - 1, c0);
-    sb0 = sb1;
-    sb1 = sb2;
+    b_cur = b_nxt;
+    b_nxt = b_nxt == (NB - 1) * UB ? 0 : b_nxt + UB;
   };
 
-  // ---- the first two slices ----
-  open_tile();
-  if constexpr (BKIND == FP8_TILES) sb0 = sbp[0];
+  // ---- the first slices: two of a, NB of b ----
+  open_a();
+  open_b();
 #pragma unroll
-  for (int q = 0; q < ND; ++q) request(0, q);
-  advance();
-  if constexpr (BKIND == FP8_TILES) sb1 = sbp[d_kb];
+  for (int n = 0; n < NB; ++n) {
+    if (n < 2) {
+      if (n > 0) advance(da, open_a);
 #pragma unroll
-  for (int q = 0; q < ND; ++q) request(STAGE, q);
+      for (int q = 0; q < DAS; ++q) request_a(n * STA, q);
+    }
+    if (n > 0) advance(db, open_b);
+#pragma unroll
+    for (int q = 0; q < DBS; ++q) request_b(B0 + n * UB, q);
+  }
   zero_acc();
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(ND) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(DAS + (NB - 1) * DBS) : "memory");
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     fa[i] = frag(ao + i * 2048);
     sa[i] = *(const float*)(lds + so + i * 64);
   }
+  if constexpr (BKIND == FP8_TILES) sb = *(const float*)(lds + co);
 #pragma unroll
   for (int j = 0; j < 3; ++j) {
     fb[j] = frag(bo + j * 2048);
@@ -463,18 +559,19 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
   }
   int ci = 0, kb = 0;
   // true after the last slice of the last tile
-  auto next = [&]() {
+  auto next = [&]() __attribute__((always_inline)) {
     if (++kb < Kb) return false;
     epilogue(tile_of(ci));
+    stores = whole;
     if (++ci == count) return true;
     zero_acc();
     kb = 0;
     return false;
   };
   for (;;) {
-    slice(fa, ga, 0, STAGE);
+    slice(fa, ga, 0, STA);
     if (next()) break;
-    slice(ga, fa, STAGE, 0);
+    slice(ga, fa, STA, 0);
     if (next()) break;
     if constexpr (ONE) {  // whole registers go round the loop (halves would be put together again)
 #pragma unroll
@@ -593,11 +690,11 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Gemm p) {
   }
 }
 
-template <int BM, int BN, int WGM, int WGN, int PER_CU, int BKIND, int OUT, bool GRP, bool EX>
+template <int BM, int BN, int WGM, int WGN, int PER_CU, int NB, int BKIND, int OUT, bool GRP, bool EX>
 hipError_t run_tile(const Fp8Gemm& p, hipStream_t s) {
   const int tiles_n = (p.n + BN - 1) / BN;
   const int tiles_m = (p.m + BM - 1) / BM + (GRP ? p.groups : 0);
-  launch_kernel((fp8_tile_kernel<BM, BN, WGM, WGN, PER_CU, BKIND, OUT, GRP, EX>),
+  launch_kernel((fp8_tile_kernel<BM, BN, WGM, WGN, PER_CU, NB, BKIND, OUT, GRP, EX>),
                 dim3(std::min(tiles_m * tiles_n, num_cus() * PER_CU)), dim3(WGM * WGN * 64), 0, s, p, tiles_m, tiles_n,
                 walk_group_m(tiles_m, tiles_n, BM, BN));
   return hipGetLastError();
@@ -614,9 +711,9 @@ template <int BKIND, int OUT, bool GRP, bool EX>
 hipError_t run_tiles(const Fp8Gemm& p, hipStream_t s) {
   if constexpr (!EX && BKIND == FP8_TILES) {
     const long long big = (long long)((p.m + 191) / 192) * ((p.n + 255) / 256);
-    if (big >= num_cus() * 3 / 4) return run_tile<192, 256, 2, 2, 1, BKIND, OUT, GRP, EX>(p, s);
+    if (big >= num_cus() * 3 / 4) return run_tile<192, 256, 2, 2, 1, 3, BKIND, OUT, GRP, EX>(p, s);
   }
-  return run_tile<128, 128, 4, 1, 2, BKIND, OUT, GRP, EX>(p, s);
+  return run_tile<128, 128, 4, 1, 2, 2, BKIND, OUT, GRP, EX>(p, s);
 }
 
 template <int BKIND, int OUT, bool GRP>
