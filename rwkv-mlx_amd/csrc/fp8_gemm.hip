@@ -250,8 +250,11 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
   Ahead da{0, 0}, db{0, 0};
   __amdgpu_buffer_rsrc_t ra, rb;
   unsigned va[DA], vb[DB];
-  const float* sbp = nullptr;  // the scales of b: of a tile's weight blocks, or columns
-  int a_m0 = 0, a_rows = 0, b_scales = 0;
+  // this wave's 64 scales of the present slice of a: of its rows (wave w < SA: rows 64·w on, further waves the last
+  // ones again), or of the tile's weight blocks; and of the present slice of b, of its columns
+  const bool blocks = !ROWS && wave >= SA;
+  const float *sap = nullptr, *sbp = nullptr;
+  unsigned sa_bytes = 0, sb_bytes = 0, sa_at = 0;
   auto open_a = [&]() __attribute__((always_inline)) {
     const Tile t = tile_of(da.i);
     int sl = lane;  // (opaque: addresses that depend on the lane alone would be kept in registers)
@@ -263,11 +266,15 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
       // rows past the end read the last one
       va[i] = (unsigned)(min(t.m0 + row, t.mlim - 1) - t.m0) * (unsigned)Kp + ((sl & 7) ^ swz(row)) * 16;
     }
-    a_m0 = t.m0;
-    a_rows = t.mlim - t.m0;
-    if constexpr (!ROWS) {
-      sbp = p.sb + ((size_t)(GRP ? min(t.g, p.groups - 1) : 0) * Nb + t.n0 / 128) * Kb;
-      b_scales = min(BN / 128, Nb - t.n0 / 128) * Kb;
+    if (blocks) {
+      const int nb = t.n0 / 128;
+      sap = p.sb + ((size_t)(GRP ? min(t.g, p.groups - 1) : 0) * Nb + nb) * Kb;
+      sa_at = BN / 128 > 1 && nb + 1 < Nb ? (sl & 1) * Kb * 4 : 0;
+      sa_bytes = 0xFFFFFFF0u;
+    } else {
+      sap = p.sa + t.m0;
+      sa_at = (min(wave, SA - 1) * 64 + sl) * 4;
+      sa_bytes = (t.mlim - t.m0) * 4;
     }
   };
   auto open_b = [&]() __attribute__((always_inline)) {
@@ -283,39 +290,39 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
     }
     if constexpr (ROWS) {
       sbp = p.sb + t.n0;
-      b_scales = min(BN, p.n - t.n0);
+      sb_bytes = min(BN, p.n - t.n0) * 4;
     }
   };
   // (past the last slice it is requested again, into a stage that nothing reads any more)
-  auto advance = [&](Ahead& d, auto open) __attribute__((always_inline)) {
-    if (d.kb + 1 < Kb) {
-      ++d.kb;
-    } else if (d.i + 1 < count) {
-      ++d.i;
-      d.kb = 0;
-      open();
+  auto advance_a = [&]() __attribute__((always_inline)) {
+    if (da.kb + 1 < Kb) {
+      ++da.kb;
+      sap += blocks ? 1 : p.m;
+    } else if (da.i + 1 < count) {
+      ++da.i;
+      da.kb = 0;
+      open_a();
+    }
+  };
+  auto advance_b = [&]() __attribute__((always_inline)) {
+    if (db.kb + 1 < Kb) {
+      ++db.kb;
+      if constexpr (ROWS) sbp += p.n;
+    } else if (db.i + 1 < count) {
+      ++db.i;
+      db.kb = 0;
+      open_b();
     }
   };
   auto request_a = [&](int stage, int q) __attribute__((always_inline)) {
     unsigned char* st = lds + stage;
-    if (q < DA) {
-      load_lds16(ra, st + (wave * DA + q) * 1024, va[q], (unsigned)da.kb * 128u);
-    } else {  // wave w: 64 rows' scales, or the weight blocks'; further waves repeat those
-      const bool b = !ROWS && wave >= SA;
-      const int c = min(wave, SA - 1), at = b ? (lane & 1) * Kb + da.kb : c * 64 + lane;
-      load_lds4(buf_rsrc(b ? sbp : p.sa + (size_t)da.kb * p.m + a_m0, (unsigned)(b ? b_scales : a_rows) * 4u),
-                st + UA + wave * 256, at * 4);
-    }
+    if (q < DA) load_lds16(ra, st + (wave * DA + q) * 1024, va[q], (unsigned)da.kb * 128u);
+    else load_lds4(buf_rsrc(sap, sa_bytes), st + UA + wave * 256, sa_at);
   };
   auto request_b = [&](int stage, int q) __attribute__((always_inline)) {
     unsigned char* st = lds + stage;
-    if (q < DB) {
-      load_lds16(rb, st + (wave * DB + q) * 1024, vb[q], (unsigned)db.kb * 128u);
-    } else {
-      const int c = min(wave, SB - 1);
-      load_lds4(buf_rsrc(sbp + (size_t)db.kb * p.n, (unsigned)b_scales * 4u), st + BN * 128 + wave * 256,
-                (c * 64 + lane) * 4);
-    }
+    if (q < DB) load_lds16(rb, st + (wave * DB + q) * 1024, vb[q], (unsigned)db.kb * 128u);
+    else load_lds4(buf_rsrc(sbp, sb_bytes), st + BN * 128 + wave * 256, (min(wave, SB - 1) * 64 + lane) * 4);
   };
 
   // ---- fragments ----
@@ -325,8 +332,9 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
   const int so = UA + (wm * WM + (lane & 15)) * 4;
   // b's scales of this wave's columns: by column, or one for all
   const int co = ROWS ? B0 + BN * 128 + (wn * WN + (lane >> 4) * 4) * 4 : UA + SA * 256 + wn * WN / 128 * 4;
-  auto frag = [&](int at) __attribute__((always_inline)) {
-    return join(*(const u32x4*)(lds + at), *(const u32x4*)(lds + (at ^ 64)));
+  const int a1 = ao ^ 64, b1 = bo ^ 64;  // the second chunk
+  auto frag = [&](int at, int at1) __attribute__((always_inline)) {
+    return join(*(const u32x4*)(lds + at), *(const u32x4*)(lds + at1));
   };
 
   f32x4 acc[MI][NI];
@@ -341,7 +349,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
   float f[MI], sa[MI], sb = 1.f;
 
   // stores of whole 16 bytes, NST of them a tile, which may be in flight through the next tile's first slice
-  constexpr int NST = MI * NI * (OUT == FP8_OUT_F32 ? 2 : 1) / 2;
+  constexpr int NST = OUT == FP8_OUT_F32 ? MI * NI : OUT == FP8_OUT_RELU2Q ? MI * (NI / 4 + 1) : MI * NI / 2;
   constexpr int WV = DAS + (NB - 2) * DBS;  // requests behind the slice that has to have landed
   static_assert(WV + NST < 64, "vmcnt range");
   const bool whole = OUT == FP8_OUT_RELU2Q || p.n % (OUT == FP8_OUT_F32 ? 4 : 8) == 0;
@@ -351,7 +359,11 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
     asm volatile("" : "+v"(el));
     if constexpr (OUT == FP8_OUT_RELU2Q) {
       const int col0 = it.n0 + wn * WN, Np = Nb * 128;
-      if (GRP && it.g == p.groups) return;
+      const int rows = GRP && it.g == p.groups ? 0 : it.mlim - it.m0;  // (rows of no range are not read)
+      const __amdgpu_buffer_rsrc_t ro =
+          buf_rsrc((unsigned char*)p.out + (size_t)it.m0 * Np, (unsigned)rows * (unsigned)Np);
+      const __amdgpu_buffer_rsrc_t rs =
+          buf_rsrc(p.out_s + (size_t)(col0 / 128) * p.m + it.m0, (unsigned)rows * 4u);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int row = it.m0 + wm * WM + i * 16 + (el & 15);
@@ -367,14 +379,27 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
         am = umax(am, (unsigned)__shfl_xor((int)am, 16));
         am = umax(am, (unsigned)__shfl_xor((int)am, 32));
         const Fp8Factors fc = fp8_factors(am);
-        if (row < it.mlim && col0 < p.n) {
-          unsigned char* q = (unsigned char*)p.out + (size_t)row * Np + col0 + (el >> 4) * 4;
+        // four blocks of 16 columns, exchanged so that a lane of 16-lane row r holds block r's 16 bytes: a store
+        // covers 64 consecutive bytes of 16 rows
 #pragma unroll
-          for (int j = 0; j < NI; ++j)
-            *(unsigned*)(q + j * 16) = fp8_pack4(acc[i][j][0] * fc.up, acc[i][j][1] * fc.up, acc[i][j][2] * fc.up,
-                                                 acc[i][j][3] * fc.up);
-          if (el < 16) p.out_s[(size_t)(col0 / 128) * p.m + row] = fc.down;
+        for (int j = 0; j < NI; j += 4) {
+          unsigned w[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            w[h] = fp8_pack4(acc[i][j + h][0] * fc.up, acc[i][j + h][1] * fc.up, acc[i][j + h][2] * fc.up,
+                             acc[i][j + h][3] * fc.up);
+          // w[h], row r: block h's bytes 4r.. -> x[..] of blocks {0, 1} and {2, 3}, then of all four
+          const auto x = __builtin_amdgcn_permlane16_swap(w[0], w[1], false, false);
+          const auto y = __builtin_amdgcn_permlane16_swap(w[2], w[3], false, false);
+          const auto lo = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+          const auto hi = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+          const unsigned off = row < it.mlim && col0 < p.n
+                                   ? (unsigned)(row - it.m0) * (unsigned)Np + col0 + (j + (el >> 4)) * 16
+                                   : kOOB;
+          __builtin_amdgcn_raw_buffer_store_b128(u32x4{lo[0], hi[0], lo[1], hi[1]}, ro, off, 0, 0);
         }
+        const unsigned soff = el < 16 && row < it.mlim && col0 < p.n ? (unsigned)(row - it.m0) * 4u : kOOB;
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, fc.down), rs, soff, 0, 0);
       }
     } else {
       typedef typename OutType<OUT>::type T;
@@ -439,86 +464,102 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
   };
 
   // One slice: a's rows in xa, its stage `cur`; the next slice's (stage nxt)
-  // into ya.  b_cur, b_nxt: b's stages.
-  int b_cur = 0, b_nxt = NB > 1 ? UB : 0;
+  // into ya.  b_cur, b_nxt: b's stages.  The fmas of a slice's last two steps
+  // follow the next slice's first two, with the factors g.
+  int b_cur = 0, b_nxt = UB;
+  f32x4 t[4];
+  f32x4 tc[ROWS ? 2 : 1];  // b's column scales of those steps
+  float g[2];
+  constexpr int NS = MI * NI;
+  static_assert(MI >= 2 && NS % 4 == 0, "four results in turn");
+  auto scale = [&](int s, float fs, const f32x4& c) __attribute__((always_inline)) {
+    const int i = s % MI, j = s / MI;
+    const f32x4 v = t[s % 4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      acc[i][j][q] = __builtin_fmaf(ROWS ? v[q] * c[q] : v[q], fs, acc[i][j][q]);
+    pin(acc[i][j]);  // (not later than here)
+  };
+  auto nothing_pending = [&]() __attribute__((always_inline)) {
+    t[2] = t[3] = f32x4{0.f, 0.f, 0.f, 0.f};
+    g[0] = g[1] = 0.f;
+    if constexpr (ROWS) tc[0] = tc[1] = t[2];
+  };
+  // the fmas that a slice leaves to the next
+  auto flush = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (ONE) asm volatile("s_nop 15" ::: "memory");
+    pin(t[2]);
+    pin(t[3]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) scale(NS - 2 + h, g[h], tc[ROWS ? h : 0]);
+  };
   auto slice = [&](i32x8 (&xa)[MI], i32x8 (&ya)[MI], int cur, int nxt) __attribute__((always_inline)) {
-    f32x4 t[3];
+    const int vb0 = bo + b_cur, vb1 = b1 + b_cur, wb0 = bo + b_nxt, wb1 = b1 + b_nxt;
 #pragma unroll
     for (int i = 0; i < MI; ++i) f[i] = sa[i] * sb;
-    f32x4 c0{1.f, 1.f, 1.f, 1.f}, c1 = c0;  // b's column scales of the step before, and of two before
-    auto scale = [&](int s, const f32x4& c) __attribute__((always_inline)) {
-      const int i = s % MI, j = s / MI;
-      pin(t[s % 3]);  // (neither before this point, nor later than it)
-      const f32x4 v = t[s % 3];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        acc[i][j][q] = __builtin_fmaf(BKIND == FP8_ROWS ? v[q] * c[q] : v[q], f[i], acc[i][j][q]);
-      pin(acc[i][j]);
-    };
+    f32x4 cj{1.f, 1.f, 1.f, 1.f}, cl = cj;  // b's column scales of this fragment, and of the one before
     auto steps = [&](auto from, auto to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = decltype(from)::value; j < decltype(to)::value; ++j) {
-      auto wb = Operand<EX>::of(fb[j & 3]);
-      const f32x4 cj = BKIND == FP8_ROWS ? cs[j & 3] : c0;
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int s = j * MI + i;
-        if constexpr (ONE) mma128_to(t[s % 3], wb, xa[i]);
-        else t[s % 3] = mma128(wb, Operand<EX>::of(xa[i]));
+      for (int s = decltype(from)::value; s < decltype(to)::value; ++s) {
+        const int j = s / MI, i = s % MI;
+        const auto w = Operand<EX>::of(fb[j & 3]);
+        if constexpr (ONE) mma128_to(t[s % 4], w, xa[i]);
+        else t[s % 4] = mma128(w, Operand<EX>::of(xa[i]));
+        // (the fmas of two steps before: not before this point)
+        pin(t[(s + 2) % 4]);
         __builtin_amdgcn_sched_barrier(0);
-        if (s >= 2) scale(s - 2, c1);
-        c1 = c0;
-        c0 = cj;
         if (i == 0) {  // fragment j + 3 of b, from NI on the next slice's
           const int e = j + 3;
-          fb[e & 3] = frag((e < NI ? b_cur : b_nxt) + bo + (e % NI) * 2048);
-          if constexpr (BKIND == FP8_ROWS)
+          fb[e & 3] = e < NI ? frag(vb0 + e * 2048, vb1 + e * 2048) : frag(wb0 + (e - NI) * 2048, wb1 + (e - NI) * 2048);
+          if constexpr (ROWS) {
+            cl = cj;
+            cj = cs[j & 3];
             cs[e & 3] = *(const f32x4*)(lds + (e < NI ? b_cur : b_nxt) + co + (e % NI) * 64);
+          }
         }
         if (j >= 1 && j < JB) {
-          constexpr int U = (JB - 1) * MI;
 #pragma unroll
           for (int q = 0; q < DAS; ++q)
-            if (q * U / DAS == s - MI) request_a(cur, q);
+            if (q * (JB - 1) * MI / DAS == s - MI) request_a(cur, q);
         }
         if (j >= JB) {
           const int u = s - JB * MI;  // of 3 · MI
           if (u % 3 == 1) {
-            ya[u / 3] = frag(nxt + ao + (u / 3) * 2048);
+            ya[u / 3] = frag(nxt + ao + (u / 3) * 2048, nxt + a1 + (u / 3) * 2048);
             sa[u / 3] = *(const float*)(lds + nxt + so + (u / 3) * 64);
-            if (BKIND == FP8_TILES && u == 1) sb = *(const float*)(lds + nxt + co);
+            if (!ROWS && u == 1) sb = *(const float*)(lds + nxt + co);
           }
 #pragma unroll
           for (int q = 0; q < DBS; ++q)
             if (q * 3 * MI / DBS == u) request_b(B0 + b_cur, q);
         }
         __builtin_amdgcn_sched_barrier(0);
+        if (s < 2) scale(NS - 2 + s, g[s], tc[ROWS ? s : 0]);
+        else scale(s - 2, f[(s - 2) % MI], i < 2 ? cl : cj);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
     };
-    steps(Int<0>{}, Int<1>{});
-    __builtin_amdgcn_sched_barrier(0);
+    steps(Int<0>{}, Int<MI>{});
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    advance(da, open_a);
-    steps(Int<1>{}, Int<JB>{});
-    __builtin_amdgcn_sched_barrier(0);
-    if (stores && OUT != FP8_OUT_RELU2Q) {  // (behind them: this slice's requests of a)
+    advance_a();
+    steps(Int<MI>{}, Int<JB * MI>{});
+    if (stores) {  // (behind them: this slice's requests of a)
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WV + NST) : "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WV) : "memory");
     }
     stores = false;
     __builtin_amdgcn_sched_barrier(0);
-    advance(db, open_b);
-    steps(Int<JB>{}, Int<NI>{});
-    if constexpr (ONE) {
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_nop 15" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
+    advance_b();
+    steps(Int<JB * MI>{}, Int<NS>{});
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      g[h] = f[MI - 2 + h];
+      if constexpr (ROWS) tc[h] = cj;
     }
-    scale(NI * MI - 2, c1);
-    scale(NI * MI - 1, c0);
     b_cur = b_nxt;
     b_nxt = b_nxt == (NB - 1) * UB ? 0 : b_nxt + UB;
   };
@@ -529,25 +570,26 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     if (n < 2) {
-      if (n > 0) advance(da, open_a);
+      if (n > 0) advance_a();
 #pragma unroll
       for (int q = 0; q < DAS; ++q) request_a(n * STA, q);
     }
-    if (n > 0) advance(db, open_b);
+    if (n > 0) advance_b();
 #pragma unroll
     for (int q = 0; q < DBS; ++q) request_b(B0 + n * UB, q);
   }
   zero_acc();
+  nothing_pending();
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(DAS + (NB - 1) * DBS) : "memory");
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    fa[i] = frag(ao + i * 2048);
+    fa[i] = frag(ao + i * 2048, a1 + i * 2048);
     sa[i] = *(const float*)(lds + so + i * 64);
   }
   if constexpr (BKIND == FP8_TILES) sb = *(const float*)(lds + co);
 #pragma unroll
   for (int j = 0; j < 3; ++j) {
-    fb[j] = frag(bo + j * 2048);
+    fb[j] = frag(bo + j * 2048, b1 + j * 2048);
     if constexpr (BKIND == FP8_ROWS) cs[j] = *(const f32x4*)(lds + co + j * 64);
   }
 
@@ -561,6 +603,8 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
   // true after the last slice of the last tile
   auto next = [&]() __attribute__((always_inline)) {
     if (++kb < Kb) return false;
+    flush();
+    nothing_pending();
     epilogue(tile_of(ci));
     stores = whole;
     if (++ci == count) return true;
