@@ -612,7 +612,8 @@ int rwkvmoe_fp8_layout(const rwkvmoe_fp8_desc* desc, const void* src, const floa
 int rwkvmoe_fp8_matmul(const rwkvmoe_fp8_desc* desc, const void* a, const float* a_scales, const void* b,
                        const float* b_scales, const int32_t* offsets, void* out, void* stream);
 
-/* Scratch bytes of rwkvmoe_fp8_linear (host only). */
+/* Scratch bytes of rwkvmoe_fp8_linear (host only); 0 for up to 64 rows, whose
+ * rounding runs in the product's launch (ws may then be NULL). */
 int rwkvmoe_fp8_linear_workspace_bytes(const rwkvmoe_fp8_desc* desc, size_t* bytes);
 
 /* x (rows, k) rounded to FP8_ROWS and multiplied with b (FP8_TILES), as

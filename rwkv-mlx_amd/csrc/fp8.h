@@ -64,7 +64,13 @@ struct Fp8Gemm {
   int out_kind;
   void* out;               // (m, n), or q (m, pad(n)) with FP8_OUT_RELU2Q
   float* out_s;            // (ceil(n / 128), m) with FP8_OUT_RELU2Q
+  // few rows (fp8_few): the rows as they are, (m, k) in the type of out with row stride ldx, instead of a and sa
+  const void* x;
+  long long ldx;
 };
+// At most this many rows: the weight's bytes bound the product.
+constexpr int kFp8FewRows = 64;
+inline bool fp8_few(int m) { return m <= kFp8FewRows; }
 hipError_t launch_fp8_gemm(const Fp8Gemm& p, hipStream_t s);
 
 // xk_j = x[t] + (shift(x)[t] - x[t]) · x_k[e] for row j of the dispatch's
@@ -97,6 +103,47 @@ RWKV_DEV unsigned fp8_pack4(float v0, float v1, float v2, float v3) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(v0, v1, 0, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(v2, v3, w, true);
   return (unsigned)w;
+}
+
+// Eight consecutive values of a row from column c (zero from `cols` on).  VEC:
+// rows are 16-byte aligned and cols is a multiple of 8.
+template <typename T, bool VEC>
+RWKV_DEV void load8(const T* row, int c, int cols, float (&v)[8]) {
+  if constexpr (VEC) {
+    if (c < cols) {
+      if constexpr (sizeof(T) == 2) {
+        Chunk<T> ch;
+        ch.raw = *(const u32x4*)(row + c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f(ch.e[i]);
+      } else {
+        const f32x4 a = *(const f32x4*)(row + c), b = *(const f32x4*)(row + c + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = a[i];
+          v[4 + i] = b[i];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f(row[c + i]) : 0.f;
+  }
+}
+
+RWKV_DEV unsigned amax8(const float (&v)[8]) {
+  unsigned a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = umax(a, abs_bits(v[i]));
+  return a;
+}
+RWKV_DEV unsigned long long pack8(const float (&v)[8], float up) {
+  const unsigned lo = fp8_pack4(v[0] * up, v[1] * up, v[2] * up, v[3] * up);
+  const unsigned hi = fp8_pack4(v[4] * up, v[5] * up, v[6] * up, v[7] * up);
+  return (unsigned long long)hi << 32 | lo;
 }
 
 }  // namespace rwkvmoe

@@ -7,107 +7,76 @@
 namespace rwkvmoe {
 namespace {
 
-// Eight consecutive values of a row from column c (zero from `cols` on).  VEC:
-// rows are 16-byte aligned and cols is a multiple of 8.
-template <typename T, bool VEC>
-RWKV_DEV void load8(const T* row, int c, int cols, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (c < cols) {
-      if constexpr (sizeof(T) == 2) {
-        Chunk<T> ch;
-        ch.raw = *(const u32x4*)(row + c);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f(ch.e[i]);
-      } else {
-        const f32x4 a = *(const f32x4*)(row + c), b = *(const f32x4*)(row + c + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = a[i];
-          v[4 + i] = b[i];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f(row[c + i]) : 0.f;
-  }
-}
-
-RWKV_DEV unsigned amax8(const float (&v)[8]) {
-  unsigned a = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) a = umax(a, abs_bits(v[i]));
-  return a;
-}
-// over the 16 lanes that share a block
+// over the 16 lanes that share a block (a DPP row)
 RWKV_DEV unsigned amax16(unsigned a) {
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) a = umax(a, (unsigned)__shfl_xor((int)a, d));
-  return a;
+  a = umax(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0x128, 0xf, 0xf, false));  // row_ror:8
+  a = umax(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0x124, 0xf, 0xf, false));
+  a = umax(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0x122, 0xf, 0xf, false));
+  return umax(a, (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, 0x121, 0xf, 0xf, false));
 }
-RWKV_DEV unsigned long long pack8(const float (&v)[8], float up) {
-  const unsigned lo = fp8_pack4(v[0] * up, v[1] * up, v[2] * up, v[3] * up);
-  const unsigned hi = fp8_pack4(v[4] * up, v[5] * up, v[6] * up, v[7] * up);
-  return (unsigned long long)hi << 32 | lo;
-}
-
-// Rows: 16 lanes a block of 128 values, a workgroup 16 rows of one slice of
-// K, so that their scales (kb, row) are 64 consecutive bytes.
+// Rows: 16 lanes a block of 128 values, a workgroup 16 rows of kRowsDeep slices
+// of K; the scales (kb, row) of the 16 rows are 64 consecutive bytes.
+// Workgroups run along K first, so that those under way together read whole
+// rows.  (Four slices a thread were slower than one: 31 us against 28 for
+// 16384 x 2048 bf16.)
+constexpr int kRowsDeep = 1;
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const T* __restrict__ x, int rows, int cols, long long ld,
                                                              unsigned char* __restrict__ q, float* __restrict__ s) {
-  const int row = blockIdx.x * 16 + (threadIdx.x >> 4), kb = blockIdx.y;
+  const int Kb = (cols + kFp8Block - 1) / kFp8Block, kw = (Kb + kRowsDeep - 1) / kRowsDeep;
+  const int row = blockIdx.x / kw * 16 + (threadIdx.x >> 4), kb0 = blockIdx.x % kw * kRowsDeep;
   if (row >= rows) return;  // (whole 16-lane blocks)
-  const int c = kb * kFp8Block + (threadIdx.x & 15) * 8;
-  float v[8];
-  load8<T, VEC>(x + (size_t)row * ld, c, cols, v);
-  const Fp8Factors f = fp8_factors(amax16(amax8(v)));
-  *(unsigned long long*)(q + (size_t)row * gridDim.y * kFp8Block + c) = pack8(v, f.up);
-  if ((threadIdx.x & 15) == 0) s[(size_t)kb * rows + row] = f.down;
+  const int c = kb0 * kFp8Block + (threadIdx.x & 15) * 8;
+  float v[kRowsDeep][8];
+#pragma unroll
+  for (int d = 0; d < kRowsDeep; ++d) load8<T, VEC>(x + (size_t)row * ld, c + d * kFp8Block, cols, v[d]);
+#pragma unroll
+  for (int d = 0; d < kRowsDeep; ++d) {
+    const Fp8Factors f = fp8_factors(amax16(amax8(v[d])));
+    if (kb0 + d >= Kb) break;
+    *(unsigned long long*)(q + (size_t)row * Kb * kFp8Block + c + d * kFp8Block) = pack8(v[d], f.up);
+    if ((threadIdx.x & 15) == 0) s[(size_t)(kb0 + d) * rows + row] = f.down;
+  }
 }
 
-// A 128 x 128 block of x by 256 threads, thread (g, c) rows 8g.. and columns
-// 8c..; its maxima by row, by column or over all go through LDS, and the 8 x 8
-// values of a thread are written as rows and as columns.
+// A 128 x 128 block of x by 512 threads, thread (g, c8) rows 4g.. and columns
+// 8·c8..; its maxima by row, by column or over all, the transposed bytes through
+// LDS so that they leave in whole lines.
 //   ROWS   q in rows (row maxima), qt in columns (column maxima)
 //   TILES  q and qt with the block's maximum
 template <typename T, bool VEC, bool TILES>
-__global__ __launch_bounds__(256) void fp8_quant_block_kernel(const T* __restrict__ x, int rows, int cols,
+__global__ __launch_bounds__(512) void fp8_quant_block_kernel(const T* __restrict__ x, int rows, int cols,
                                                               long long ld, unsigned char* __restrict__ q,
                                                               float* __restrict__ s, unsigned char* __restrict__ qt,
                                                               float* __restrict__ st) {
-  __shared__ unsigned cmax[16][132];
-  const int tid = threadIdx.x, c8 = tid & 15, g = tid >> 4;
+  constexpr int R = 4, P = 33;  // rows of a thread; dwords between columns of the transposed bytes
+  __shared__ unsigned tile[128 * P];
+  __shared__ unsigned cmax[8][128];
+  __shared__ float cup[128];
+  const int tid = threadIdx.x, c8 = tid & 15, g = tid >> 4, wave = tid >> 6;
   const int rb = blockIdx.y, kb = blockIdx.x, grp = blockIdx.z;
   const int Kb = gridDim.x, Rb = gridDim.y;
-  const int r0 = rb * kFp8Block + g * 8, c0 = kb * kFp8Block + c8 * 8;
+  const int r0 = rb * kFp8Block + g * R, c0 = kb * kFp8Block + c8 * 8;
   const T* xg = x + (size_t)grp * rows * ld;
-  float v[8][8];
+  float v[R][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (r0 + i < rows) {
-      load8<T, VEC>(xg + (size_t)(r0 + i) * ld, c0, cols, v[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    }
-  }
-  Fp8Factors fr[8], fc[8];
+  for (int i = 0; i < R; ++i)
+    load8<T, VEC>(xg + (size_t)min(r0 + i, rows - 1) * ld, c0, r0 + i < rows ? cols : 0, v[i]);
+  float up[R];
   if constexpr (TILES) {
     unsigned a = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a = umax(a, amax8(v[i]));
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) a = umax(a, (unsigned)__shfl_xor((int)a, d));
-    if ((tid & 63) == 0) cmax[0][tid >> 6] = a;
+    for (int i = 0; i < R; ++i) a = umax(a, amax8(v[i]));
+    a = amax16(a);
+    a = umax(a, (unsigned)__shfl_xor((int)a, 16));
+    a = umax(a, (unsigned)__shfl_xor((int)a, 32));
+    if ((tid & 63) == 0) cmax[0][wave] = a;
     __syncthreads();
-    a = umax(umax(cmax[0][0], cmax[0][1]), umax(cmax[0][2], cmax[0][3]));
+#pragma unroll
+    for (int w = 0; w < 8; ++w) a = umax(a, cmax[0][w]);
     const Fp8Factors f = fp8_factors(a);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) fr[i] = fc[i] = f;
+    for (int i = 0; i < R; ++i) up[i] = f.up;
     if (tid == 0) {
       if (q) s[((size_t)grp * Rb + rb) * Kb + kb] = f.down;
       if (qt) st[((size_t)grp * Kb + kb) * Rb + rb] = f.down;
@@ -115,9 +84,10 @@ __global__ __launch_bounds__(256) void fp8_quant_block_kernel(const T* __restric
   } else {
     if (q) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        fr[i] = fp8_factors(amax16(amax8(v[i])));
-        if (c8 == 0 && r0 + i < rows) s[(size_t)kb * rows + r0 + i] = fr[i].down;
+      for (int i = 0; i < R; ++i) {
+        const Fp8Factors f = fp8_factors(amax16(amax8(v[i])));
+        up[i] = f.up;
+        if (c8 == 0 && r0 + i < rows) s[(size_t)kb * rows + r0 + i] = f.down;
       }
     }
     if (qt) {
@@ -125,37 +95,44 @@ __global__ __launch_bounds__(256) void fp8_quant_block_kernel(const T* __restric
       for (int j = 0; j < 8; ++j) {
         unsigned a = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a = umax(a, abs_bits(v[i][j]));
-        cmax[g][c8 * 8 + j] = a;
+        for (int i = 0; i < R; ++i) a = umax(a, abs_bits(v[i][j]));
+        a = umax(a, (unsigned)__shfl_xor((int)a, 16));
+        a = umax(a, (unsigned)__shfl_xor((int)a, 32));
+        if ((tid & 63) < 16) cmax[wave][c8 * 8 + j] = a;
       }
       __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      if (tid < 128) {
         unsigned a = 0;
 #pragma unroll
-        for (int h = 0; h < 16; ++h) a = umax(a, cmax[h][c8 * 8 + j]);
-        fc[j] = fp8_factors(a);
-        if (g == 0 && c0 + j < cols) st[(size_t)rb * cols + c0 + j] = fc[j].down;
+        for (int w = 0; w < 8; ++w) a = umax(a, cmax[w][tid]);
+        const Fp8Factors f = fp8_factors(a);
+        cup[tid] = f.up;
+        if (kb * kFp8Block + tid < cols) st[(size_t)rb * cols + kb * kFp8Block + tid] = f.down;
       }
+      __syncthreads();
     }
   }
   if (q) {
     unsigned char* qg = q + (size_t)grp * rows * Kb * kFp8Block;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < R; ++i)
       if (r0 + i < rows)
-        *(unsigned long long*)(qg + ((size_t)(r0 + i) * Kb + kb) * kFp8Block + c8 * 8) = pack8(v[i], fr[i].up);
+        *(unsigned long long*)(qg + ((size_t)(r0 + i) * Kb + kb) * kFp8Block + c8 * 8) = pack8(v[i], up[i]);
   }
   if (qt) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float u = TILES ? up[0] : cup[c8 * 8 + j];
+      tile[(c8 * 8 + j) * P + g] = fp8_pack4(v[0][j] * u, v[1][j] * u, v[2][j] * u, v[3][j] * u);
+    }
+    __syncthreads();
     unsigned char* tg = qt + (size_t)grp * cols * Rb * kFp8Block;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c0 + j < cols) {
-        float w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = v[i][j];
-        *(unsigned long long*)(tg + ((size_t)(c0 + j) * Rb + rb) * kFp8Block + g * 8) = pack8(w, fc[j].up);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const int c = i * 16 + (tid >> 5), d = tid & 31;
+      if (kb * kFp8Block + c < cols)
+        *(unsigned*)(tg + ((size_t)(kb * kFp8Block + c) * Rb + rb) * kFp8Block + d * 4) = tile[c * P + d];
+    }
   }
 }
 
@@ -200,31 +177,37 @@ bool vec_rows(const Fp8Quant& p) {
   return p.cols % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (p.ld * sizeof(T)) % 16 == 0;
 }
 
-// Token t's mixed row for expert e, 8 values from column c, in fp32 (one
-// rounding, to e4m3, follows).
+// Token t's mixed row for expert e in fp32 (one rounding, to e4m3, follows);
+// as the rows kernel, kMixDeep slices of K a workgroup.
+constexpr int kMixDeep = 1;
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void fp8_mix_kernel(const T* __restrict__ x, const T* __restrict__ xprev,
                                                       const T* __restrict__ mu, const int* __restrict__ perm,
                                                       const int* __restrict__ inds, const int* __restrict__ off,
                                                       int nk, int T_, int C, int E, int k,
                                                       unsigned char* __restrict__ q, float* __restrict__ s) {
-  const int j = blockIdx.x * 16 + (threadIdx.x >> 4), kb = blockIdx.y;
+  const int Kb = (C + kFp8Block - 1) / kFp8Block, kw = (Kb + kMixDeep - 1) / kMixDeep;
+  const int j = blockIdx.x / kw * 16 + (threadIdx.x >> 4), kb0 = blockIdx.x % kw * kMixDeep;
   if (j >= off[E]) return;  // (assignments of no expert are not in perm)
   const int a = perm[j], t = a / k, e = inds[a];
-  const int c = kb * kFp8Block + (threadIdx.x & 15) * 8;
-  float v[8], pv[8], m[8];
-  load8<T, VEC>(x + (size_t)t * C, c, C, v);
-  if (t % T_ > 0) load8<T, VEC>(x + (size_t)(t - 1) * C, c, C, pv);
-  else if (xprev) load8<T, VEC>(xprev + (size_t)(t / T_) * C, c, C, pv);
-  else
+  const int c = kb0 * kFp8Block + (threadIdx.x & 15) * 8;
+  const T* prev = t % T_ > 0 ? x + (size_t)(t - 1) * C : xprev ? xprev + (size_t)(t / T_) * C : nullptr;
+  float v[kMixDeep][8], pv[kMixDeep][8], m[kMixDeep][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) pv[i] = 0.f;
-  load8<T, VEC>(mu + (size_t)e * C, c, C, m);
+  for (int d = 0; d < kMixDeep; ++d) {
+    load8<T, VEC>(x + (size_t)t * C, c + d * kFp8Block, C, v[d]);
+    load8<T, VEC>(prev ? prev : x, c + d * kFp8Block, prev ? C : 0, pv[d]);
+    load8<T, VEC>(mu + (size_t)e * C, c + d * kFp8Block, C, m[d]);
+  }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = v[i] + (pv[i] - v[i]) * m[i];
-  const Fp8Factors f = fp8_factors(amax16(amax8(v)));
-  *(unsigned long long*)(q + (size_t)j * gridDim.y * kFp8Block + c) = pack8(v, f.up);
-  if ((threadIdx.x & 15) == 0) s[(size_t)kb * nk + j] = f.down;
+  for (int d = 0; d < kMixDeep; ++d) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[d][i] = v[d][i] + (pv[d][i] - v[d][i]) * m[d][i];
+    const Fp8Factors f = fp8_factors(amax16(amax8(v[d])));
+    if (kb0 + d >= Kb) break;
+    *(unsigned long long*)(q + (size_t)j * Kb * kFp8Block + c + d * kFp8Block) = pack8(v[d], f.up);
+    if ((threadIdx.x & 15) == 0) s[(size_t)(kb0 + d) * nk + j] = f.down;
+  }
 }
 
 // Four columns of a token a thread.
@@ -262,11 +245,11 @@ hipError_t launch_fp8_quant_rows(const Fp8Quant& p, hipStream_t s) {
     const bool v = vec_rows<T>(p);
     if (p.qt) {
       launch_kernel(v ? fp8_quant_block_kernel<T, true, false> : fp8_quant_block_kernel<T, false, false>,
-                    dim3(Kb, fp8_blocks(p.rows), 1), dim3(256), 0, s, (const T*)p.x, p.rows, p.cols, p.ld, p.q, p.s,
+                    dim3(Kb, fp8_blocks(p.rows), 1), dim3(512), 0, s, (const T*)p.x, p.rows, p.cols, p.ld, p.q, p.s,
                     p.qt, p.st);
     } else {
       launch_kernel(v ? fp8_quant_rows_kernel<T, true> : fp8_quant_rows_kernel<T, false>,
-                    dim3((p.rows + 15) / 16, Kb), dim3(256), 0, s, (const T*)p.x, p.rows, p.cols, p.ld, p.q, p.s);
+                    dim3((Kb + kRowsDeep - 1) / kRowsDeep * ((p.rows + 15) / 16)), dim3(256), 0, s, (const T*)p.x, p.rows, p.cols, p.ld, p.q, p.s);
     }
   });
   return mark(hipGetLastError(), "fp8_quant", s);
@@ -275,7 +258,7 @@ hipError_t launch_fp8_quant_rows(const Fp8Quant& p, hipStream_t s) {
 hipError_t launch_fp8_quant_tiles(const Fp8Quant& p, hipStream_t s) {
   RWKV_DISPATCH_DTYPE(p.dtype, T, {
     launch_kernel(vec_rows<T>(p) ? fp8_quant_block_kernel<T, true, true> : fp8_quant_block_kernel<T, false, true>,
-                  dim3(fp8_blocks(p.cols), fp8_blocks(p.rows), p.groups), dim3(256), 0, s, (const T*)p.x, p.rows,
+                  dim3(fp8_blocks(p.cols), fp8_blocks(p.rows), p.groups), dim3(512), 0, s, (const T*)p.x, p.rows,
                   p.cols, p.ld, p.q, p.s, p.qt, p.st);
   });
   return mark(hipGetLastError(), "fp8_quant", s);
@@ -293,7 +276,7 @@ hipError_t launch_fp8_mix(int dtype, const void* x, const void* xprev, const voi
   const int nk = N * k;
   RWKV_DISPATCH_DTYPE(dtype, T, {
     const bool v = C % 8 == 0 && ((uintptr_t)x | (uintptr_t)xprev | (uintptr_t)mu) % 16 == 0;
-    launch_kernel(v ? fp8_mix_kernel<T, true> : fp8_mix_kernel<T, false>, dim3((nk + 15) / 16, fp8_blocks(C)),
+    launch_kernel(v ? fp8_mix_kernel<T, true> : fp8_mix_kernel<T, false>, dim3((fp8_blocks(C) + kMixDeep - 1) / kMixDeep * ((nk + 15) / 16)),
                   dim3(256), 0, st, (const T*)x, (const T*)xprev, (const T*)mu, perm, inds, off, nk, T_, C, E, k, q, s);
   });
   return mark(hipGetLastError(), "fp8_mix", st);

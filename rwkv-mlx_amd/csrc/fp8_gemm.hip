@@ -631,23 +631,28 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
 // ---- few rows -------------------------------------------------------------------
 
 // At most a few rows to a weight: the weight's bytes are what counts, each is
-// read once from memory straight into registers.  Eight waves: NT blocks of 16
-// columns, each of them shared by 8 / NT waves that take every (8 / NT)-th
-// slice of K and are summed through LDS.
-template <int NT, int BKIND, int OUT, bool GRP>
+// read once from memory straight into registers.  Eight waves, each with CT
+// blocks of 16 columns; NT waves side by side, and 8 / NT share their columns,
+// take every (8 / NT)-th slice of K and are summed through LDS.
+// RAW: the rows come unrounded, and every wave rounds the blocks it multiplies
+// itself, which saves a launch (one bf16 row by 8192 x 2048: kernels of 2.6 and
+// 5.4 us against one of 8.2, but a pass from the host 12.9 against 8.6); what
+// that costs in every workgroup is shared by its CT blocks.  VEC: their loads are 16 bytes.  D: slices whose loads are
+// under way together (past the end: the last slice again).
+template <int NT, int CT, int D, int BKIND, int OUT, bool GRP, bool RAW, bool VEC>
 __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Gemm p) {
-  constexpr int KS = 8 / NT;
-  static_assert(OUT != FP8_OUT_RELU2Q || NT == 8, "whole blocks of 128 columns");
-  __shared__ __attribute__((aligned(16))) f32x4 part[KS > 1 ? 8 * 64 : 1];
+  constexpr int KS = 8 / NT, COLS = NT * CT * 16;
+  static_assert(OUT != FP8_OUT_RELU2Q || (NT == 8 && CT == 1), "whole blocks of 128 columns");
+  __shared__ __attribute__((aligned(16))) f32x4 part[KS > 1 ? CT * 8 * 64 : 1];
   __shared__ unsigned amax[8][16];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nt = wave % NT, ks = wave / NT;
-  const int Kb = (p.k + 127) / 128, Kp = Kb * 128;
-  const int c0 = blockIdx.x * NT * 16 + nt * 16, g = blockIdx.y;
+  const int Kb = (p.k + 127) / 128, Kp = Kb * 128, Nb = (p.n + 127) / 128;
+  const int c0 = blockIdx.x * COLS + nt * CT * 16, g = blockIdx.y;
   int lo = 0, hi = p.m;
   if constexpr (GRP) {
-    // as find_range: from the largest offset before
+    // as Ranges: from the largest offset before
     for (int i = lane; i <= g; i += 64) lo = max(lo, i > 0 ? p.off[i] : 0);
     hi = g == p.groups ? p.m : p.off[g + 1];
 #pragma unroll
@@ -657,60 +662,122 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Gemm p) {
     if (g == p.groups) {  // rows of no range
       if constexpr (OUT != FP8_OUT_RELU2Q) {
         typedef typename OutType<OUT>::type T;
-        for (int i = tid; i < (hi - lo) * NT * 16; i += 512) {
-          const int row = lo + i / (NT * 16), c = blockIdx.x * NT * 16 + i % (NT * 16);
+        for (int i = tid; i < (hi - lo) * COLS; i += 512) {
+          const int row = lo + i / COLS, c = blockIdx.x * COLS + i % COLS;
           if (c < p.n) ((T*)p.out)[(size_t)row * p.n + c] = from_f<T>(0.f);
         }
       }
       return;
     }
   }
-  const unsigned char* brow = p.b + ((size_t)g * p.n + min(c0 + (lane & 15), p.n - 1)) * Kp + (lane >> 4) * 16;
-  const float* sbp = BKIND == FP8_TILES
-                         ? p.sb + ((size_t)g * ((p.n + 127) / 128) + min(c0 / 128, (p.n + 127) / 128 - 1)) * Kb
-                         : p.sb;
+  const unsigned char* brow[CT];
+  const float* sbp[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = c0 + ct * 16;
+    brow[ct] = p.b + ((size_t)g * p.n + min(c + (lane & 15), p.n - 1)) * Kp + (lane >> 4) * 16;
+    sbp[ct] = BKIND == FP8_TILES ? p.sb + ((size_t)g * Nb + min(c / 128, Nb - 1)) * Kb : p.sb;
+  }
   for (int m0 = lo; m0 < hi; m0 += 16) {
     const int row = m0 + (lane & 15), arow = min(row, hi - 1);
-    const unsigned char* ar = p.a + (size_t)arow * Kp + (lane >> 4) * 16;
-    f32x4 acc{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-    for (int kb = ks; kb < Kb; kb += KS) {
-      const i32x8 fb = join(*(const u32x4*)(brow + kb * 128), *(const u32x4*)(brow + kb * 128 + 64));
-      const i32x8 fa = join(*(const u32x4*)(ar + kb * 128), *(const u32x4*)(ar + kb * 128 + 64));
-      const float sa = p.sa[(size_t)kb * p.m + arow];
-      const f32x4 t = mma128(widen(fb), widen(fa));
-      if constexpr (BKIND == FP8_TILES) {
-        const float f = sa * sbp[kb];
+    f32x4 acc[CT];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[q] = __builtin_fmaf(t[q], f, acc[q]);
+    for (int ct = 0; ct < CT; ++ct) acc[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = ks; k0 < Kb; k0 += KS * D) {
+      u32x4 w[D][CT][2];
+#pragma unroll
+      for (int d = 0; d < D; ++d)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const unsigned char* bp = brow[ct] + min(k0 + d * KS, Kb - 1) * 128;
+          w[d][ct][0] = *(const u32x4*)bp;
+          w[d][ct][1] = *(const u32x4*)(bp + 64);
+        }
+      i32x8 fa[D];
+      float sa[D];
+      if constexpr (RAW) {
+        // this lane's 16 values of either chunk; the block's others lie in the lanes 16, 32 and 48 further on
+        typedef typename OutType<OUT>::type T;
+        const T* xr = (const T*)p.x + (size_t)arow * p.ldx;
+        float v[D][4][8];
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            load8<T, VEC>(xr, min(k0 + d * KS, Kb - 1) * 128 + (lane >> 4) * 16 + (h >> 1) * 64 + (h & 1) * 8, p.k,
+                          v[d][h]);
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+          unsigned am = 0;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) am = umax(am, amax8(v[d][h]));
+          am = umax(am, (unsigned)__shfl_xor((int)am, 16));
+          am = umax(am, (unsigned)__shfl_xor((int)am, 32));
+          const Fp8Factors fx = fp8_factors(am);
+          sa[d] = fx.down;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const unsigned long long q = pack8(v[d][h], fx.up);
+            fa[d][h * 2] = (int)(unsigned)q;
+            fa[d][h * 2 + 1] = (int)(unsigned)(q >> 32);
+          }
+        }
       } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          acc[q] = __builtin_fmaf(t[q] * sbp[(size_t)kb * p.n + min(c0 + (lane >> 4) * 4 + q, p.n - 1)], sa, acc[q]);
+        for (int d = 0; d < D; ++d) {
+          const int kb = min(k0 + d * KS, Kb - 1);
+          const unsigned char* ar = p.a + (size_t)arow * Kp + kb * 128 + (lane >> 4) * 16;
+          fa[d] = join(*(const u32x4*)ar, *(const u32x4*)(ar + 64));
+          sa[d] = p.sa[(size_t)kb * p.m + arow];
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const int kb = k0 + d * KS;
+        if (kb >= Kb) break;
+        const Wide wa = widen(fa[d]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const f32x4 t = mma128(widen(join(w[d][ct][0], w[d][ct][1])), wa);
+          if constexpr (BKIND == FP8_TILES) {
+            const float f = sa[d] * sbp[ct][kb];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[ct][q] = __builtin_fmaf(t[q], f, acc[ct][q]);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              acc[ct][q] = __builtin_fmaf(
+                  t[q] * sbp[ct][(size_t)kb * p.n + min(c0 + ct * 16 + (lane >> 4) * 4 + q, p.n - 1)], sa[d],
+                  acc[ct][q]);
+          }
+        }
       }
     }
     if constexpr (KS > 1) {
-      part[wave * 64 + lane] = acc;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) part[(ct * 8 + wave) * 64 + lane] = acc[ct];
       __syncthreads();
       if (ks == 0) {
 #pragma unroll
-        for (int s = 1; s < KS; ++s) {
-          const f32x4 v = part[(s * NT + nt) * 64 + lane];
+        for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) acc[q] += v[q];
-        }
+          for (int s = 1; s < KS; ++s) {
+            const f32x4 v = part[(ct * 8 + s * NT + nt) * 64 + lane];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[ct][q] += v[q];
+          }
       }
       __syncthreads();
       if (ks != 0) continue;
     }
-    const int c = c0 + (lane >> 4) * 4;
     if constexpr (OUT == FP8_OUT_RELU2Q) {
+      const int c = c0 + (lane >> 4) * 4;
       unsigned am = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float z = acc[q] < 0.f ? 0.f : acc[q];
-        acc[q] = c + q < p.n ? z * z : 0.f;
-        am = umax(am, abs_bits(acc[q]));
+        const float z = acc[0][q] < 0.f ? 0.f : acc[0][q];  // (a NaN stays one)
+        acc[0][q] = c + q < p.n ? z * z : 0.f;
+        am = umax(am, abs_bits(acc[0][q]));
       }
       am = umax(am, (unsigned)__shfl_xor((int)am, 16));
       am = umax(am, (unsigned)__shfl_xor((int)am, 32));
@@ -720,16 +787,20 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Gemm p) {
       for (int s = 0; s < 8; ++s) am = umax(am, amax[s][lane & 15]);
       __syncthreads();
       const Fp8Factors fc = fp8_factors(am);
-      const int Np = (p.n + 127) / 128 * 128;
       if (row < hi) {
-        *(unsigned*)((unsigned char*)p.out + (size_t)row * Np + c) =
-            fp8_pack4(acc[0] * fc.up, acc[1] * fc.up, acc[2] * fc.up, acc[3] * fc.up);
+        *(unsigned*)((unsigned char*)p.out + (size_t)row * Nb * 128 + c) =
+            fp8_pack4(acc[0][0] * fc.up, acc[0][1] * fc.up, acc[0][2] * fc.up, acc[0][3] * fc.up);
         if (wave == 0 && lane < 16) p.out_s[(size_t)blockIdx.x * p.m + row] = fc.down;
       }
     } else {
       typedef typename OutType<OUT>::type T;
-      const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-      if (row < hi) store4<T>((T*)p.out + (size_t)row * p.n, c, p.n, p.n % 4 == 0, v);
+      if (row < hi) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const float v[4] = {acc[ct][0], acc[ct][1], acc[ct][2], acc[ct][3]};
+          store4<T>((T*)p.out + (size_t)row * p.n, c0 + ct * 16 + (lane >> 4) * 4, p.n, p.n % 4 == 0, v);
+        }
+      }
     }
   }
 }
@@ -744,25 +815,56 @@ hipError_t run_tile(const Fp8Gemm& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int NT, int BKIND, int OUT, bool GRP>
+template <int NT, int CT, int D, int BKIND, int OUT, bool GRP>
 hipError_t run_few(const Fp8Gemm& p, hipStream_t s) {
-  launch_kernel((fp8_few_kernel<NT, BKIND, OUT, GRP>), dim3((p.n + NT * 16 - 1) / (NT * 16), GRP ? p.groups + 1 : 1),
-                dim3(512), 0, s, p);
+  const dim3 grid((p.n + NT * CT * 16 - 1) / (NT * CT * 16), GRP ? p.groups + 1 : 1), block(512);
+  if constexpr (OUT != FP8_OUT_RELU2Q && BKIND == FP8_TILES) {
+    if (p.x) {
+      typedef typename OutType<OUT>::type T;
+      const bool vec = p.k % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (p.ldx * sizeof(T)) % 16 == 0;
+      if (vec) launch_kernel((fp8_few_kernel<NT, CT, D, BKIND, OUT, GRP, true, true>), grid, block, 0, s, p);
+      else launch_kernel((fp8_few_kernel<NT, CT, D, BKIND, OUT, GRP, true, false>), grid, block, 0, s, p);
+      return hipGetLastError();
+    }
+  }
+  launch_kernel((fp8_few_kernel<NT, CT, D, BKIND, OUT, GRP, false, true>), grid, block, 0, s, p);
   return hipGetLastError();
+}
+
+template <int BKIND, int OUT, bool GRP>
+hipError_t run_few_rows(const Fp8Gemm& p, hipStream_t s) {
+  if constexpr (OUT == FP8_OUT_RELU2Q) {
+    return run_few<8, 1, 2, BKIND, OUT, GRP>(p, s);
+  } else {
+    // workgroups of 64 columns where they fill the card, so that a row's block is rounded once for four blocks of
+    // columns (16 weights of 4096 x 1024, 24 bf16 rows: 19 us against 42); slices of K a wave: one or more
+    const long long groups = GRP ? std::min(p.groups, p.m) : 1;
+    const bool wide = (p.n + 63) / 64 * groups >= 2 * num_cus();
+    const bool deep = p.k > 8 * 128;
+    if (wide) return deep ? run_few<1, 4, 2, BKIND, OUT, GRP>(p, s) : run_few<1, 4, 1, BKIND, OUT, GRP>(p, s);
+    return deep ? run_few<1, 1, 2, BKIND, OUT, GRP>(p, s) : run_few<1, 1, 1, BKIND, OUT, GRP>(p, s);
+  }
 }
 
 template <int BKIND, int OUT, bool GRP, bool EX>
 hipError_t run_tiles(const Fp8Gemm& p, hipStream_t s) {
+  // The wide tile reads 0.73 of the 128 x 128 tile's bytes a product, but only
+  // one fits a CU: nothing runs beside a tile's first and last slices, and a
+  // round of tiles that fills few CUs costs a whole one.  Measured (us, 128 x
+  // 128 against 192 x 256): 16384 x 8192 x 2048 311, 288; 3000 x 4096 x 8192
+  // 117, 105; 8192 x 8192 x 1024 94, 101; 4096 x 1024 x 4096 (96 wide tiles) 27, 44.
   if constexpr (!EX && BKIND == FP8_TILES) {
-    const long long big = (long long)((p.m + 191) / 192) * ((p.n + 255) / 256);
-    if (big >= num_cus() * 3 / 4) return run_tile<192, 256, 2, 2, 1, 3, BKIND, OUT, GRP, EX>(p, s);
+    const long long cus = num_cus(), tiles_n = (p.n + 255) / 256;
+    const long long tiles = ((p.m + 191) / 192 + (GRP ? p.groups / 2 : 0)) * tiles_n;
+    if (p.k > 11 * 128 && tiles * 5 >= (tiles + cus - 1) / cus * cus * 4)
+      return run_tile<192, 256, 2, 2, 1, 3, BKIND, OUT, GRP, EX>(p, s);
   }
   return run_tile<128, 128, 4, 1, 2, 2, BKIND, OUT, GRP, EX>(p, s);
 }
 
 template <int BKIND, int OUT, bool GRP>
 hipError_t run(const Fp8Gemm& p, hipStream_t s) {
-  if (p.m <= 64) return run_few<OUT == FP8_OUT_RELU2Q ? 8 : 1, BKIND, OUT, GRP>(p, s);
+  if (fp8_few(p.m)) return run_few_rows<BKIND, OUT, GRP>(p, s);
   if constexpr (OUT == FP8_OUT_F32 || OUT == FP8_OUT_RELU2Q) {
     if (p.exact) return run_tiles<BKIND, OUT, GRP, true>(p, s);
   }

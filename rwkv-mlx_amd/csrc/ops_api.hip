@@ -75,6 +75,8 @@ int check_fp8(const rwkvmoe_fp8_desc* d, bool product) {
   if (d->block != RWKVMOE_FP8_ROWS && d->block != RWKVMOE_FP8_TILES) return RWKVMOE_ERR_MODE;
   if (d->rows < 0 || d->rows > kMaxRows || d->k < 1 || d->k > kMaxK || d->groups < 0 || d->groups > kMaxGroups)
     return RWKVMOE_ERR_SHAPE;
+  // (the workgroups of a launch: 16 rows of one slice of k)
+  if ((d->rows / 16 + 1ll) * fp8_blocks(d->k) >= 0x7fffffffll) return RWKVMOE_ERR_SHAPE;
   if (product) {
     if (d->n < 1 || d->n > kMaxK) return RWKVMOE_ERR_SHAPE;
     // (the tiles of a launch)
@@ -120,7 +122,8 @@ int check_experts(const rwkvmoe_desc* d, ExpertsLayout* L) {
   if (d->top_k < 1 || d->top_k > std::min(d->n_experts, 8)) return RWKVMOE_ERR_TOPK;
   if (d->flags & ~(RWKVMOE_HAS_PREV | RWKVMOE_ADD_RESIDUAL)) return RWKVMOE_ERR_FLAGS;
   const long long N = (long long)d->batch * d->seq_len, nk = N * d->top_k;
-  if (nk > kMaxRows || (nk / kFp8Block + 1 + d->n_experts) * fp8_blocks(std::max(d->d_ffn, d->d_model)) >= 0x7fffffffll)
+  if (nk > kMaxRows || (nk / 16 + 1) * fp8_blocks(d->d_model) >= 0x7fffffffll ||
+      (nk / kFp8Block + 1 + d->n_experts) * fp8_blocks(std::max(d->d_ffn, d->d_model)) >= 0x7fffffffll)
     return RWKVMOE_ERR_SHAPE;
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -217,7 +220,7 @@ int rwkvmoe_fp8_matmul(const rwkvmoe_fp8_desc* desc, const void* a, const float*
 int rwkvmoe_fp8_linear_workspace_bytes(const rwkvmoe_fp8_desc* desc, size_t* bytes) {
   TRY(check_fp8(desc, true));
   if (!bytes) return RWKVMOE_ERR_NULL_PTR;
-  *bytes = up256(q_bytes(desc->rows, desc->k)) + up256(s_bytes(desc->rows, desc->k));
+  *bytes = fp8_few(desc->rows) ? 0 : up256(q_bytes(desc->rows, desc->k)) + up256(s_bytes(desc->rows, desc->k));
   return RWKVMOE_OK;
 }
 
@@ -229,6 +232,13 @@ int rwkvmoe_fp8_linear(const rwkvmoe_fp8_desc* desc, const void* x, const void* 
   if (desc->rows == 0) return RWKVMOE_OK;
   TRY(need(x, elem_size(desc->dtype))); TRY(need(b, 16)); TRY(need(b_scales, 4)); TRY(need(out, 16));
   if (desc->groups) TRY(need(offsets, 4));
+  if (fp8_few(desc->rows)) {  // rounded in the product's launch
+    Fp8Gemm g = gemm_of(desc, nullptr, nullptr, b, b_scales, offsets, out);
+    g.x = x;
+    g.ldx = desc->stride;
+    HIPTRY(launch_fp8_gemm(g, (hipStream_t)stream));
+    return RWKVMOE_OK;
+  }
   const size_t qb = up256(q_bytes(desc->rows, desc->k)), sb = up256(s_bytes(desc->rows, desc->k));
   if (!ws || ws_bytes < qb + sb || !aligned(ws, 256)) return RWKVMOE_ERR_WORKSPACE;
   unsigned char* q = (unsigned char*)ws;

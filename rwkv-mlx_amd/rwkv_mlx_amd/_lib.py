@@ -391,25 +391,35 @@ def check(status: int, where: str) -> None:
         raise RwkvMoeError(status, where)
 
 
-class _Here:
-    """The current device already."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
 def on_device(device: torch.device):
-    """A context in which `device` is current: a launch on a default stream
-    goes to the current device."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
+    """A context in which `device` is current (a launch on a default stream goes
+    to the current device), or None where it is already."""
+    return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def launch(fn, where: str, device: torch.device, *args) -> None:
+    """fn(*args, current stream of `device`) with `device` current; raise
+    RwkvMoeError on a non-zero status."""
+    ctx = on_device(device)
+    if ctx is None:
+        st = fn(*args, current_stream(device))
+    else:
+        with ctx:
+            st = fn(*args, current_stream(device))
+    if st != 0:
+        raise RwkvMoeError(st, where)
+
+
+@lru_cache(maxsize=1024)
+def route_desc(*dims):
+    """A rwkvmoe_route_desc that calls of these sizes share, by reference."""
+    return ctypes.byref(RouteDesc(*dims))
+
+
+@lru_cache(maxsize=4096)
+def fp8_desc(*dims):
+    """A rwkvmoe_fp8_desc that calls of these sizes share, by reference."""
+    return ctypes.byref(Fp8Desc(*dims))
 
 
 @lru_cache(maxsize=1024)

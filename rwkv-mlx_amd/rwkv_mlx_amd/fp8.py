@@ -61,8 +61,7 @@ def _stride(x: torch.Tensor) -> int:
 
 
 def _call(name: str, x: torch.Tensor, *args) -> None:
-    with _lib.on_device(x.device):
-        _lib.check(getattr(_lib.lib(), name)(*args, _lib.current_stream(x.device)), name)
+    _lib.launch(getattr(_lib.lib(), name), name, x.device, *args)
 
 
 def fp8_quantize(x: torch.Tensor, transposed: bool = False, rows: bool = True):
@@ -81,8 +80,8 @@ def fp8_quantize(x: torch.Tensor, transposed: bool = False, rows: bool = True):
         q, s = _bytes(R, _blocks(K) * BLOCK, device=dev), _f32(_blocks(K), R, device=dev)
     if transposed:
         qt, st = _bytes(K, _blocks(R) * BLOCK, device=dev), _f32(_blocks(R), K, device=dev)
-    desc = _lib.Fp8Desc(R, 0, K, 0, _code(x, "fp8_quantize"), _lib.FP8_ROWS, _stride(x))
-    _call("rwkvmoe_fp8_quantize", x, ctypes.byref(desc), x.data_ptr(), _lib.ptr(q), _lib.ptr(s), _lib.ptr(qt),
+    desc = _lib.fp8_desc(R, 0, K, 0, _code(x, "fp8_quantize"), _lib.FP8_ROWS, _stride(x))
+    _call("rwkvmoe_fp8_quantize", x, desc, x.data_ptr(), _lib.ptr(q), _lib.ptr(s), _lib.ptr(qt),
           _lib.ptr(st))
     return tuple(t for t in (q, s, qt, st) if t is not None)
 
@@ -126,8 +125,8 @@ class Fp8Weight:
         w = w.detach().contiguous()
         out = cls._empty(w.shape, w.device, transposed)
         N, K = w.shape[-2:]
-        desc = _lib.Fp8Desc(N, 0, K, out.groups, code, _lib.FP8_TILES, K)
-        _call("rwkvmoe_fp8_quantize", w, ctypes.byref(desc), w.data_ptr(), out.q.data_ptr(), out.scale.data_ptr(),
+        desc = _lib.fp8_desc(N, 0, K, out.groups, code, _lib.FP8_TILES, K)
+        _call("rwkvmoe_fp8_quantize", w, desc, w.data_ptr(), out.q.data_ptr(), out.scale.data_ptr(),
               _lib.ptr(out.q_t), _lib.ptr(out.scale_t))
         return out
 
@@ -145,8 +144,8 @@ class Fp8Weight:
                              f"expected, got {tuple(scale.shape)} on {scale.device}")
         q, scale = q.detach().contiguous(), scale.detach().to(torch.float32).contiguous()
         out = cls._empty(q.shape, q.device, transposed)
-        desc = _lib.Fp8Desc(0, N, K, out.groups, _lib.F32, _lib.FP8_TILES, K)
-        _call("rwkvmoe_fp8_layout", q, ctypes.byref(desc), q.data_ptr(), scale.data_ptr(), out.q.data_ptr(),
+        desc = _lib.fp8_desc(0, N, K, out.groups, _lib.F32, _lib.FP8_TILES, K)
+        _call("rwkvmoe_fp8_layout", q, desc, q.data_ptr(), scale.data_ptr(), out.q.data_ptr(),
               out.scale.data_ptr(), _lib.ptr(out.q_t), _lib.ptr(out.scale_t))
         return out
 
@@ -161,20 +160,20 @@ def _product(x, N, K, groups, code, q, scale, offsets, dtype):
     """x (R, K) rounded and multiplied with a weight in 8 bits: (R, N)."""
     R = x.shape[0]
     out = torch.empty(R, N, dtype=dtype, device=x.device)
-    desc = _lib.Fp8Desc(R, N, K, groups, code, _lib.FP8_TILES, _stride(x))
+    desc = _lib.fp8_desc(R, N, K, groups, code, _lib.FP8_TILES, _stride(x))
     nbytes = _lib.fp8_linear_bytes(R, N, K, groups, code)
     # (from torch's allocator: a captured graph keeps its own)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    _call("rwkvmoe_fp8_linear", x, ctypes.byref(desc), x.data_ptr(), q.data_ptr(), scale.data_ptr(),
-          _lib.ptr(offsets), out.data_ptr(), ws.data_ptr(), nbytes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    _call("rwkvmoe_fp8_linear", x, desc, x.data_ptr(), q.data_ptr(), scale.data_ptr(),
+          None if offsets is None else offsets.data_ptr(), out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
 def _matmul(aq, a_s, bq, b_s, M, N, K, block, dtype, like):
     """The product of two matrices in 8 bits, (M, K) and (N, K)."""
     out = torch.empty(M, N, dtype=dtype, device=aq.device)
-    desc = _lib.Fp8Desc(M, N, K, 0, _lib.TORCH_DTYPE_CODE[dtype], block, K)
-    _call("rwkvmoe_fp8_matmul", like, ctypes.byref(desc), aq.data_ptr(), a_s.data_ptr(), bq.data_ptr(),
+    desc = _lib.fp8_desc(M, N, K, 0, _lib.TORCH_DTYPE_CODE[dtype], block, K)
+    _call("rwkvmoe_fp8_matmul", like, desc, aq.data_ptr(), a_s.data_ptr(), bq.data_ptr(),
           b_s.data_ptr(), None, out.data_ptr())
     return out
 

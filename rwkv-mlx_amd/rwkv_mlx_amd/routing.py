@@ -9,8 +9,6 @@ softmax case without groups and bias).
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
@@ -28,9 +26,8 @@ def _route(plan, logits, bias):
     desc, shape, k = plan
     inds = torch.empty(*shape, k, dtype=torch.int32, device=logits.device)
     gates = torch.empty(*shape, k, dtype=torch.float32, device=logits.device)
-    with _lib.on_device(logits.device):
-        _lib.check(_lib.lib().rwkvmoe_route(ctypes.byref(desc), logits.data_ptr(), _lib.ptr(bias), inds.data_ptr(),
-                                            gates.data_ptr(), _lib.current_stream(logits.device)), "rwkvmoe_route")
+    _lib.launch(_lib.lib().rwkvmoe_route, "rwkvmoe_route", logits.device, desc, logits.data_ptr(),
+                None if bias is None else bias.data_ptr(), inds.data_ptr(), gates.data_ptr())
     return inds, gates
 
 
@@ -41,19 +38,20 @@ class _RouteFunction(torch.autograd.Function):
         ctx.save_for_backward(logits, inds, gates)
         ctx.desc = plan[0]
         ctx.mark_non_differentiable(inds)
+        ctx.set_materialize_grads(False)  # (no zeros for inds)
         return inds, gates
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_inds, d_gates):
+        if d_gates is None:
+            return None, None, None
         logits, inds, gates = ctx.saved_tensors
         d_gates = d_gates.to(torch.float32).contiguous()
         # (dense, whatever the strides of logits)
         d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        with _lib.on_device(logits.device):
-            _lib.check(_lib.lib().rwkvmoe_route_backward(
-                ctypes.byref(ctx.desc), logits.data_ptr(), inds.data_ptr(), gates.data_ptr(), d_gates.data_ptr(),
-                d_logits.data_ptr(), _lib.current_stream(logits.device)), "rwkvmoe_route_backward")
+        _lib.launch(_lib.lib().rwkvmoe_route_backward, "rwkvmoe_route_backward", logits.device, ctx.desc,
+                    logits.data_ptr(), inds.data_ptr(), gates.data_ptr(), d_gates.data_ptr(), d_logits.data_ptr())
         return d_logits, None, None
 
 
@@ -87,7 +85,8 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None = 
         if bias.shape != (E,) or bias.device != logits.device:
             raise ValueError(f"route_topk: bias ({E},) on {logits.device} expected, got {tuple(bias.shape)} on "
                              f"{bias.device}")
-        bias = bias.detach().to(torch.float32).contiguous()
+        if bias.requires_grad or bias.dtype is not torch.float32 or not bias.is_contiguous():
+            bias = bias.detach().to(torch.float32).contiguous()
     shape = logits.shape[:-1]
     # rows of one stride are read in place
     if logits.dim() == 2 and logits.stride(1) == 1 and logits.stride(0) >= E:
@@ -96,12 +95,12 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None = 
         flat = logits.reshape(-1, E).contiguous()
     rows = flat.shape[0]
     stride = flat.stride(0) if rows > 1 else E
-    desc = _lib.RouteDesc(rows, E, top_k, n_groups, n_groups if top_groups is None else top_groups,
-                          _lib.TORCH_DTYPE_CODE[logits.dtype], SCORES[score], GROUP_SCORES[group_score],
-                          _lib.ROUTE_RENORM if renormalize else 0, scale, max(stride, E))
+    desc = _lib.route_desc(rows, E, top_k, n_groups, n_groups if top_groups is None else top_groups,
+                           _lib.TORCH_DTYPE_CODE[logits.dtype], SCORES[score], GROUP_SCORES[group_score],
+                           _lib.ROUTE_RENORM if renormalize else 0, scale, max(stride, E))
     plan = (desc, shape, top_k)
     if rows == 0:  # nothing to launch; the options are checked all the same
-        _lib.check(_lib.lib().rwkvmoe_route(ctypes.byref(desc), None, None, None, None, None), "rwkvmoe_route")
+        _lib.check(_lib.lib().rwkvmoe_route(desc, None, None, None, None, None), "rwkvmoe_route")
         return (torch.empty(*shape, top_k, dtype=torch.int32, device=logits.device),
                 logits.new_zeros((*shape, top_k), dtype=torch.float32) + logits.sum().to(torch.float32) * 0
                 if logits.requires_grad else

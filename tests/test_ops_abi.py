@@ -101,7 +101,9 @@ def test_fp8_pointers_and_workspace():
     assert lib.rwkvmoe_fp8_matmul(ref(fp8_desc(n=0)), *[FAKE] * 6, None) == -2
     b = ctypes.c_size_t(0)
     assert lib.rwkvmoe_fp8_linear_workspace_bytes(ref(d), None) == -4
-    assert lib.rwkvmoe_fp8_linear_workspace_bytes(ref(d), ref(b)) == 0 and b.value == 512 + 256
+    assert lib.rwkvmoe_fp8_linear_workspace_bytes(ref(d), ref(b)) == 0 and b.value == 0
+    d = fp8_desc(rows=65)
+    assert lib.rwkvmoe_fp8_linear_workspace_bytes(ref(d), ref(b)) == 0 and b.value == 65 * 128 + 128 + 512
     lin = lambda desc, ws, n: lib.rwkvmoe_fp8_linear(ref(desc), FAKE, FAKE, FAKE, None, FAKE, ws, n, None)
     assert lin(d, None, b.value) == -6 and lin(d, FAKE, b.value - 1) == -6 and lin(d, FAKE + 16, b.value) == -6
     assert lin(fp8_desc(block=0), FAKE, 1 << 20) == -9 and lin(fp8_desc(stride=8), FAKE, 1 << 20) == -2
