@@ -582,7 +582,7 @@ enum rwkvmoe_fp8_block { RWKVMOE_FP8_ROWS = 0, RWKVMOE_FP8_TILES = 1 };
 
 typedef struct rwkvmoe_fp8_desc {
   int32_t rows;    /* rows of x and out, 0..8388480 */
-  int32_t n;       /* columns of out = rows of the weight (the products) */
+  int32_t n;       /* columns of out = rows of the weight (the products), 1..4194304 */
   int32_t k;       /* columns of x and of the weight, 1..8388608 */
   int32_t groups;  /* 0: one matrix; else 1..1024 weights of the same shape */
   int32_t dtype;   /* enum rwkvmoe_dtype of x and out */

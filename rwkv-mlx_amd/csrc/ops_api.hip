@@ -68,6 +68,7 @@ int check_route(const rwkvmoe_route_desc* d, Route* r) {
 // ---- 8-bit products ----
 
 constexpr int kMaxRows = 65535 * kFp8Block, kMaxK = 1 << 23, kMaxGroups = 1024;
+constexpr int kMaxN = 1 << 22;  // (a tile's rows of out lie within 4 GB)
 
 int check_fp8(const rwkvmoe_fp8_desc* d, bool product) {
   if (!d) return RWKVMOE_ERR_NULL_DESC;
@@ -78,7 +79,7 @@ int check_fp8(const rwkvmoe_fp8_desc* d, bool product) {
   // (the workgroups of a launch: 16 rows of one slice of k)
   if ((d->rows / 16 + 1ll) * fp8_blocks(d->k) >= 0x7fffffffll) return RWKVMOE_ERR_SHAPE;
   if (product) {
-    if (d->n < 1 || d->n > kMaxK) return RWKVMOE_ERR_SHAPE;
+    if (d->n < 1 || d->n > kMaxN) return RWKVMOE_ERR_SHAPE;
     // (the tiles of a launch)
     if ((long long)(fp8_blocks(d->rows) + d->groups) * fp8_blocks(d->n) >= 0x7fffffffll) return RWKVMOE_ERR_SHAPE;
     if (d->groups && d->block != RWKVMOE_FP8_TILES) return RWKVMOE_ERR_MODE;
@@ -116,8 +117,8 @@ struct ExpertsLayout {
 int check_experts(const rwkvmoe_desc* d, ExpertsLayout* L) {
   if (!d) return RWKVMOE_ERR_NULL_DESC;
   TRY(check_dtype(d->dtype));
-  if (d->batch < 0 || d->seq_len < 0 || d->d_model < 4 || d->d_model % 4 || d->d_model > kMaxK || d->d_ffn < 1 ||
-      d->d_ffn > kMaxK || d->n_experts < 1 || d->n_experts > 64)
+  if (d->batch < 0 || d->seq_len < 0 || d->d_model < 4 || d->d_model % 4 || d->d_model > kMaxN || d->d_ffn < 1 ||
+      d->d_ffn > kMaxN || d->n_experts < 1 || d->n_experts > 64)
     return RWKVMOE_ERR_SHAPE;
   if (d->top_k < 1 || d->top_k > std::min(d->n_experts, 8)) return RWKVMOE_ERR_TOPK;
   if (d->flags & ~(RWKVMOE_HAS_PREV | RWKVMOE_ADD_RESIDUAL)) return RWKVMOE_ERR_FLAGS;

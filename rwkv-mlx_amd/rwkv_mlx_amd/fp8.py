@@ -291,7 +291,7 @@ def fp8_grouped_linear(x: torch.Tensor, weight: Fp8Weight, offsets: torch.Tensor
     E, N, K = weight.shape
     _check_x(x, K, weight.device, "fp8_grouped_linear")
     if x.dim() != 2:
-        raise ValueError(f"fp8_grouped_linear: x ({'R'}, {K}) expected, got {tuple(x.shape)}")
+        raise ValueError(f"fp8_grouped_linear: x (R, {K}) expected, got {tuple(x.shape)}")
     if offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or offsets.device != x.device:
         raise ValueError(f"fp8_grouped_linear: offsets ({E + 1},) int32 on {x.device} expected, got "
                          f"{tuple(offsets.shape)} {offsets.dtype} on {offsets.device}")
@@ -379,6 +379,19 @@ class Fp8MoE_CMix(nn.Module):
         """From a ``MoE_CMix`` on the GPU; `router` replaces the layer's."""
         return cls(layer.router if router is None else router, layer.x_k.reshape(layer.n_experts, -1),
                    Fp8Weight.quantize(layer.expert_key), Fp8Weight.quantize(layer.expert_val))
+
+    def _apply(self, fn, recurse=True):
+        # a cast (.half(), .to(dtype)) is for the router and x_k: the weights go through it as integers
+        views = {f"{n}_q": torch.uint8 for n in ("key", "value")}
+        views.update({f"{n}_scale": torch.int32 for n in ("key", "value")})
+        was = {n: self._buffers[n].dtype for n in views}
+        for n, dt in views.items():
+            self._buffers[n] = self._buffers[n].view(dt)
+        try:
+            return super()._apply(fn, recurse)
+        finally:
+            for n, dt in was.items():
+                self._buffers[n] = self._buffers[n].view(dt)
 
     def forward(self, x: torch.Tensor, x_prev: torch.Tensor | None = None, residual: torch.Tensor | None = None):
         """(out, aux_loss, z_loss), as MoE_CMix's forward."""

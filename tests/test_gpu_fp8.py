@@ -392,3 +392,73 @@ def test_refusals(device):
             (lambda: ex(residual=x), ValueError), (lambda: ex(gates=torch.zeros(1, 4, 1)), ValueError)):
         with pytest.raises(err):
             call()
+
+
+def test_a_layer_keeps_its_weights_through_casts(device):
+    torch.manual_seed(1)
+    moe = MoE_CMix(RWKVConfig(n_embd=64, dim_ffn=128), 0, 4, 2).to(device)
+    with torch.no_grad():
+        moe.expert_val.normal_(0, 0.1)
+    layer = Fp8MoE_CMix.from_moe(moe)
+    q, s = layer.key_q.clone(), layer.value_scale.clone()
+    layer.half()
+    assert layer.x_k.dtype == torch.float16 and layer.router.gate.weight.dtype == torch.float16
+    assert torch.equal(layer.key_q.view(torch.uint8), q.view(torch.uint8)) and torch.equal(layer.value_scale, s)
+    out, _, _ = layer(torch.randn(1, 5, 64, device=device).half())
+    assert out.dtype == torch.float16 and torch.isfinite(out).all()
+    again = Fp8MoE_CMix.from_moe(moe).half()
+    again.load_state_dict(layer.state_dict())
+    assert torch.equal(again.key_q.view(torch.uint8), layer.key_q.view(torch.uint8))
+
+
+def test_offsets_past_32_bits(device):
+    """x, its 8-bit form and the product lie past 4 GB: the last rows are the
+    ones that they are on their own."""
+    R, K, N = 2_200_000, 2048, 520
+    x = torch.empty(R, K, dtype=torch.bfloat16, device=device).normal_()
+    tail = x[-200:].clone()
+    q, s, qt, st = fp8_quantize(x, transposed=True)
+    q1, s1 = fp8_quantize(tail)
+    assert q.numel() > 1 << 32
+    assert torch.equal(q[-200:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[:, -200:], s1)
+    last = R // 128 * 128 - 128  # the last whole block of rows
+    qt1 = fp8_quantize(x[last:last + 128].clone(), transposed=True, rows=False)[0]
+    assert torch.equal(qt[:, last:last + 128].contiguous().view(torch.uint8), qt1.view(torch.uint8))
+    del q, s, qt, st
+    h = Fp8Weight.quantize(rand((N, K), "bf16", 1).to(device))
+    y = fp8_linear(x, h)
+    assert torch.equal(y[-200:], fp8_linear(tail, h))
+    he = Fp8Weight.quantize(rand((2, N, K), "bf16", 1).to(device))
+    off = torch.tensor([0, 7, R - 100], dtype=torch.int32, device=device)
+    y = fp8_grouped_linear(x, he, off)
+    h1 = Fp8Weight.quantize(rand((2, N, K), "bf16", 1)[1].to(device))
+    assert torch.equal(y[-200:-100], fp8_linear(tail[:100], h1)) and (y[-100:] == 0).all()
+
+
+def test_gradients_in_a_graph(device):
+    x = rand((150, 256), "bf16", 1).to(device).requires_grad_(True)
+    w = rand((200, 256), "bf16", 2).to(device).requires_grad_(True)
+    he = Fp8Weight.quantize(rand((3, 200, 256), "bf16", 3).to(device), transposed=True)
+    off = torch.tensor([0, 40, 90, 150], dtype=torch.int32, device=device)
+    dy = rand((150, 200), "bf16", 4).to(device)
+
+    def step():
+        a = torch.autograd.grad(fp8_linear(x, w), (x, w), dy)
+        b = torch.autograd.grad(fp8_grouped_linear(x, he, off), x, dy)
+        return (*a, *b)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for seed in range(3):
+        with torch.no_grad():
+            x.copy_(rand((150, 256), "bf16", seed + 20))
+            dy.copy_(rand((150, 200), "bf16", seed + 30))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))

@@ -188,3 +188,67 @@ def test_group_router(device):
     r.update_balance(inds, 0.5)
     load = np.bincount(inds.cpu().numpy().ravel(), minlength=16)
     assert (np.sign(load.mean() - load) * 0.5 == r.balance_bias.cpu().numpy()).all()
+
+
+def test_route_past_32_bits(device):
+    R, E = 4_300_000, 256
+    l = torch.empty(R, E, device=device).normal_()
+    tail = l[-300:].clone().requires_grad_(True)
+    assert l.numel() * 4 > 1 << 32
+    b = torch.randn(E, device=device) * 0.1
+    kw = dict(bias=b, score="sigmoid", n_groups=8, top_groups=4, group_score="top2")
+    l.requires_grad_(True)
+    inds, gates = route_topk(l, 8, **kw)
+    i1, g1 = route_topk(tail, 8, **kw)
+    assert torch.equal(inds[-300:], i1) and torch.equal(gates[-300:], g1)
+    dg = torch.empty(R, 8, device=device).normal_()
+    (d,) = torch.autograd.grad(gates, l, dg)
+    (d1,) = torch.autograd.grad(g1, tail, dg[-300:])
+    assert torch.equal(d[-300:], d1)
+
+
+def test_route_rows_of_near_ties(device):
+    """Scores closer than fp32 resolves, many of them in a row: 16 and 64 lanes
+    a row, a few and more than a wave settles, and at the border of groups."""
+    rng = np.random.default_rng(0)
+    for R in (70, 4100):
+        base = rng.normal(size=(R, 1))
+        l = (base + rng.integers(0, 4, (R, 64)) * 2.0 ** -22).astype(np.float32)
+        l[::3] = rng.normal(size=l[::3].shape)
+        l[1::3, ::5] += rng.normal(size=l[1::3, ::5].shape).astype(np.float32)
+        b = (rng.integers(0, 3, 64) * 2.0 ** -25).astype(np.float32)
+        for score in ("sigmoid", "softmax"):
+            for k, G, tg, bias in ((3, 1, 1, True), (6, 8, 2, True), (12, 4, 2, True), (5, 8, 3, False), (14, 2, 2, True)):
+                kw = dict(score=score, n_groups=G, top_groups=tg, group_score="top2")
+                inds, gates = route_topk(torch.from_numpy(l).to(device), k,
+                                         bias=torch.from_numpy(b).to(device) if bias else None, **kw)
+                wi, wg = O.route(l.astype(np.float64), k, bias=b if bias else None, **kw)
+                # (softmax's scores are sums' quotients: the last bit of 64 may fall either way, so their values
+                # are compared, and the experts where no two scores lie within 2^-48)
+                s, _ = O.route_scores(l.astype(np.float64), score)
+                val = s + (b if bias else 0)
+                got = np.take_along_axis(val, inds.cpu().numpy().astype(np.int64), 1)
+                want = np.take_along_axis(val, wi, 1)
+                assert (np.abs(got - want) <= 2.0 ** -48 * np.abs(want)).all()
+                if score == "sigmoid" and G == 1:
+                    assert (inds.cpu().numpy() == wi).all()
+
+
+def test_route_gradient_in_a_graph(device):
+    l = torch.randn(500, 64, device=device, requires_grad=True)
+    dg = torch.randn(500, 4, device=device)
+    step = lambda: torch.autograd.grad(route_topk(l, 4, score="sigmoid", n_groups=4, top_groups=2)[1], l, dg)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for seed in range(3):
+        with torch.no_grad():
+            l.copy_(torch.randn(500, 64, generator=torch.Generator().manual_seed(seed)))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, step())
