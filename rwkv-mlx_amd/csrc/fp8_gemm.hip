@@ -853,10 +853,13 @@ hipError_t run_tiles(const Fp8Gemm& p, hipStream_t s) {
   // round of tiles that fills few CUs costs a whole one.  Measured (us, 128 x
   // 128 against 192 x 256): 16384 x 8192 x 2048 311, 288; 3000 x 4096 x 8192
   // 117, 105; 8192 x 8192 x 1024 94, 101; 4096 x 1024 x 4096 (96 wide tiles) 27, 44.
+  // Hidden rows are half the bytes of 16-bit results, so their epilogue pays for
+  // itself sooner: 32496 rows of 32
+  // experts x 4096 x 1024 285, 249.
   if constexpr (!EX && BKIND == FP8_TILES) {
     const long long cus = num_cus(), tiles_n = (p.n + 255) / 256;
     const long long tiles = ((p.m + 191) / 192 + (GRP ? p.groups / 2 : 0)) * tiles_n;
-    if (p.k > 11 * 128 && tiles * 5 >= (tiles + cus - 1) / cus * cus * 4)
+    if (p.k > (OUT == FP8_OUT_RELU2Q ? 7 : 11) * 128 && tiles * 5 >= (tiles + cus - 1) / cus * cus * 4)
       return run_tile<192, 256, 2, 2, 1, 3, BKIND, OUT, GRP, EX>(p, s);
   }
   return run_tile<128, 128, 4, 1, 2, 2, BKIND, OUT, GRP, EX>(p, s);
