@@ -530,7 +530,7 @@ enum rwkvmoe_group_score { RWKVMOE_GROUP_MAX = 0, RWKVMOE_GROUP_TOP2 = 1 };
 #define RWKVMOE_ROUTE_RENORM 1
 
 typedef struct rwkvmoe_route_desc {
-  int32_t rows;          /* tokens (0: nothing is done) */
+  int32_t rows;          /* tokens, 0..67108800 (0: nothing is done) */
   int32_t n_experts;     /* E, 1..512 */
   int32_t top_k;         /* k, 1..min(32, top_groups · E / n_groups) */
   int32_t n_groups;      /* G, 1..64, a divisor of E (1: no groups) */
@@ -577,7 +577,8 @@ int rwkvmoe_route_backward(const rwkvmoe_route_desc* desc, const void* logits, c
  *           (ceil(R / 128), Kb) for blocks of 128 x 128 (FP8_TILES)
  * and stands for q · scale.  Rounding a block with a = max(|v|, 2^-100):
  * scale = fp32(a / 448), q = e4m3(v · fp32(448 / a)), to nearest even.  A NaN
- * or an infinity makes its block NaN. */
+ * or an infinity makes its block NaN.  A launch has fewer than 2^32 threads:
+ * matrices of more than about 2^35 values are refused. */
 enum rwkvmoe_fp8_block { RWKVMOE_FP8_ROWS = 0, RWKVMOE_FP8_TILES = 1 };
 
 typedef struct rwkvmoe_fp8_desc {

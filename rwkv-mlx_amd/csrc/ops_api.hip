@@ -35,12 +35,18 @@ int need(const void* p, size_t a) {
 int maybe(const void* p, size_t a) { return !p || aligned(p, a) ? RWKVMOE_OK : RWKVMOE_ERR_ALIGN; }
 int check_dtype(int dt) { return dt >= RWKVMOE_F32 && dt <= RWKVMOE_BF16 ? RWKVMOE_OK : RWKVMOE_ERR_DTYPE; }
 
+// A launch has fewer than 2^32 threads, of 256 a workgroup (of 512, where
+// fewer workgroups are launched).
+constexpr long long kMaxBlocks = (1ll << 24) - 1;
+
 // ---- routing ----
+
+constexpr int kMaxRouteRows = (1 << 26) - 64;  // (up to 64 threads a row)
 
 int check_route(const rwkvmoe_route_desc* d, Route* r) {
   if (!d) return RWKVMOE_ERR_NULL_DESC;
   TRY(check_dtype(d->dtype));
-  if (d->rows < 0 || d->rows > 0x7fffffff - 64 || d->n_experts < 1 || d->n_experts > kRouteMaxE)
+  if (d->rows < 0 || d->rows > kMaxRouteRows || d->n_experts < 1 || d->n_experts > kRouteMaxE)
     return RWKVMOE_ERR_SHAPE;
   if (d->n_groups < 1 || d->n_groups > kRouteMaxGroups || d->n_experts % d->n_groups || d->top_groups < 1 ||
       d->top_groups > d->n_groups || d->logits_stride < d->n_experts)
@@ -77,7 +83,7 @@ int check_fp8(const rwkvmoe_fp8_desc* d, bool product) {
   if (d->rows < 0 || d->rows > kMaxRows || d->k < 1 || d->k > kMaxK || d->groups < 0 || d->groups > kMaxGroups)
     return RWKVMOE_ERR_SHAPE;
   // (the workgroups of a launch: 16 rows of one slice of k)
-  if ((d->rows / 16 + 1ll) * fp8_blocks(d->k) >= 0x7fffffffll) return RWKVMOE_ERR_SHAPE;
+  if ((d->rows / 16 + 1ll) * fp8_blocks(d->k) > kMaxBlocks) return RWKVMOE_ERR_SHAPE;
   if (product) {
     if (d->n < 1 || d->n > kMaxN) return RWKVMOE_ERR_SHAPE;
     // (the tiles of a launch)
@@ -123,7 +129,8 @@ int check_experts(const rwkvmoe_desc* d, ExpertsLayout* L) {
   if (d->top_k < 1 || d->top_k > std::min(d->n_experts, 8)) return RWKVMOE_ERR_TOPK;
   if (d->flags & ~(RWKVMOE_HAS_PREV | RWKVMOE_ADD_RESIDUAL)) return RWKVMOE_ERR_FLAGS;
   const long long N = (long long)d->batch * d->seq_len, nk = N * d->top_k;
-  if (nk > kMaxRows || (nk / 16 + 1) * fp8_blocks(d->d_model) >= 0x7fffffffll ||
+  if (nk > kMaxRows || (nk / 16 + 1) * fp8_blocks(d->d_model) > kMaxBlocks ||
+      N * (d->d_model / 4) > kMaxBlocks * 256 ||
       (nk / kFp8Block + 1 + d->n_experts) * fp8_blocks(std::max(d->d_ffn, d->d_model)) >= 0x7fffffffll)
     return RWKVMOE_ERR_SHAPE;
   size_t off = 0;

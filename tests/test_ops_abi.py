@@ -154,3 +154,24 @@ def test_python_refuses_cpu_tensors():
             call()
     with pytest.raises(TypeError):
         fp8_grouped_linear(x, x, torch.zeros(2, dtype=torch.int32))
+
+
+def test_launches_stay_below_2_to_32_threads():
+    """More rows than one launch has threads for are refused on the host."""
+    lib, ref, b = L.lib(), ctypes.byref, ctypes.c_size_t(0)
+    d = route_desc(rows=(1 << 26) - 63)
+    assert lib.rwkvmoe_route(ref(d), FAKE, None, FAKE, FAKE, None) == -2
+    assert lib.rwkvmoe_route_backward(ref(d), FAKE, FAKE, FAKE, FAKE, FAKE, None) == -2
+    big = dict(k=8192, stride=8192)  # 64 slices: 2^18 workgroups of 16 rows are too many
+    d = fp8_desc(rows=1 << 22, **big)
+    assert lib.rwkvmoe_fp8_quantize(ref(d), FAKE, FAKE, FAKE, None, None, None) == -2
+    assert lib.rwkvmoe_fp8_linear_workspace_bytes(ref(d), ref(b)) == -2
+    assert lib.rwkvmoe_fp8_linear_workspace_bytes(ref(fp8_desc(rows=(1 << 22) - 64, **big)), ref(b)) == 0
+    e = L.Desc()
+    e.batch, e.seq_len, e.d_ffn, e.n_experts, e.top_k = 1, 1 << 22, 128, 8, 1
+    for c in (4096, 8192):  # tokens x C / 4 threads
+        e.d_model = c
+        assert lib.rwkvmoe_fp8_experts_workspace_bytes(ref(e), ref(b)) == -2
+    e.seq_len = (1 << 22) - 64
+    e.d_model = 4096
+    assert lib.rwkvmoe_fp8_experts_workspace_bytes(ref(e), ref(b)) == 0
