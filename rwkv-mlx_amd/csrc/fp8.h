@@ -1,7 +1,7 @@
 // 8-bit block-scaled operands (e4m3, one fp32 scale for each 128 values of a
-// row or each 128 x 128 block of a weight) and the launchers of fp8.hip,
-// fp8_gemm.hip and fp8_experts.hip.  Shapes and pointers are checked by
-// fp8_api.hip before any of these is called.
+// row or each 128 x 128 block of a weight) and the launchers of fp8.hip and
+// fp8_gemm.hip.  Shapes and pointers are checked by ops_api.hip before any of
+// these is called.
 //
 // A block with a = max |v| (at least 2^-100, so that both factors below are
 // normal fp32 numbers) is held as q = e4m3(v · fp32(448 / a)), rounded to

@@ -109,6 +109,11 @@ RWKV_DEV void store4(T* row, int c, int n, bool vec, const float (&v)[4]) {
   }
 }
 
+// Four values at any multiple of their size: one store.
+template <typename T> struct Four {
+  T e[4];
+};
+
 template <int OUT> struct OutType { typedef float type; };
 template <> struct OutType<FP8_OUT_F16> { typedef f16 type; };
 template <> struct OutType<FP8_OUT_BF16> { typedef bf16 type; };
@@ -193,7 +198,7 @@ template <int N> struct Int { static constexpr int value = N; };
 //     slice after next, and the next slice has to have landed.
 //   * Workgroups are persistent and the slices run on across tiles.
 template <int BM, int BN, int WGM, int WGN, int PER_CU, int NB, int BKIND, int OUT, bool GRP, bool EX>
-__global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_tile_kernel(Fp8Gemm p, int tiles_m,
+__global__ __launch_bounds__(WGM * WGN * 64, (PER_CU * WGM * WGN + 3) / 4) void fp8_tile_kernel(Fp8Gemm p, int tiles_m,
                                                                                      int tiles_n, int group_m) {
   constexpr int NW = WGM * WGN;
   constexpr int WM = BM / WGM, WN = BN / WGN, MI = WM / 16, NI = WN / 16;
@@ -451,12 +456,19 @@ __global__ __launch_bounds__(WGM * WGN * 64, PER_CU * WGM * WGN / 4) void fp8_ti
           if (row < rows) {
             T* o = (T*)p.out + (size_t)(it.m0 + row) * p.n;
 #pragma unroll
-            for (int j = 0; j < NI; ++j)
+            for (int j = 0; j < NI; ++j) {
+              const int c = col0 + j * 16 + (el >> 4) * 4;
+              Four<T> w;
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const int c = col0 + j * 16 + (el >> 4) * 4 + q;
-                if (c < p.n) o[c] = from_f<T>(none ? 0.f : acc[i][j][q]);
+              for (int q = 0; q < 4; ++q) w.e[q] = from_f<T>(none ? 0.f : acc[i][j][q]);
+              if (c + 4 <= p.n) {
+                *(Four<T>*)(o + c) = w;
+              } else {
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+                  if (c + q < p.n) o[c + q] = w.e[q];
               }
+            }
           }
         }
       }
@@ -854,13 +866,22 @@ hipError_t run_tiles(const Fp8Gemm& p, hipStream_t s) {
   // 128 against 192 x 256): 16384 x 8192 x 2048 311, 288; 3000 x 4096 x 8192
   // 117, 105; 8192 x 8192 x 1024 94, 101; 4096 x 1024 x 4096 (96 wide tiles) 27, 44.
   // Hidden rows are half the bytes of 16-bit results, so their epilogue pays for
-  // itself sooner: 32496 rows of 32
-  // experts x 4096 x 1024 285, 249.
-  if constexpr (!EX && BKIND == FP8_TILES) {
-    const long long cus = num_cus(), tiles_n = (p.n + 255) / 256;
-    const long long tiles = ((p.m + 191) / 192 + (GRP ? p.groups / 2 : 0)) * tiles_n;
-    if (p.k > (OUT == FP8_OUT_RELU2Q ? 7 : 11) * 128 && tiles * 5 >= (tiles + cus - 1) / cus * cus * 4)
-      return run_tile<192, 256, 2, 2, 1, 3, BKIND, OUT, GRP, EX>(p, s);
+  // itself sooner: 32496 rows of 32 experts x 4096 x 1024 285, 249.
+  // Where 128 x 128 tiles leave half of the CUs idle, 64 x 128 ones read more
+  // but are sooner done (us, 128 x 128 against 64 x 128): 200 x 4096 x 1024 9.4,
+  // 8.1; 1024 x 2048 x 1024 9.4, 8.6; with more tiles 2048 x 2048 x 1024 10.4,
+  // 11.6; 300 x 8192 x 8192 45.8, 51.8.
+  if constexpr (BKIND == FP8_TILES) {
+    const long long cus = num_cus();
+    auto tiles = [&](int bm, int bn) {
+      return ((p.m + bm - 1) / bm + (GRP ? p.groups / 2 : 0)) * (long long)((p.n + bn - 1) / bn);
+    };
+    if constexpr (!EX) {
+      const long long wide = tiles(192, 256);
+      if (p.k > (OUT == FP8_OUT_RELU2Q ? 7 : 11) * 128 && wide * 5 >= (wide + cus - 1) / cus * cus * 4)
+        return run_tile<192, 256, 2, 2, 1, 3, BKIND, OUT, GRP, EX>(p, s);
+    }
+    if (tiles(128, 128) * 2 <= cus) return run_tile<64, 128, 2, 1, 3, 2, BKIND, OUT, GRP, EX>(p, s);
   }
   return run_tile<128, 128, 4, 1, 2, 2, BKIND, OUT, GRP, EX>(p, s);
 }

@@ -462,3 +462,57 @@ def test_gradients_in_a_graph(device):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("N,K", [(2690, 1500), (2688, 1500), (2691, 300)])
+def test_tiles_of_every_size_give_the_same_bits(device, dtype, N, K):
+    """A row's sums take one order whatever tile holds it: 64 x 128 with 300
+    rows, 128 x 128 with 1500, 192 x 256 with 3840 (16-bit results, K > 11
+    blocks), and the first of these is held against the formula."""
+    x, w = rand((3840, K), dtype, 1, 0.3), rand((N, K), dtype, 2, 0.3)
+    h, xd = Fp8Weight.quantize(w.to(device)), x.to(device)
+    all_rows = fp8_linear(xd, h)
+    for r in (65, 300, 1500):
+        assert torch.equal(fp8_linear(xd[:r], h), all_rows[:r]), r
+    assert torch.equal(fp8_linear(xd[3000:], h), all_rows[3000:])
+    close(all_rows[:100], O.held_rows(*O.quantize_rows(x[:100].float().numpy())),
+          O.held_tiles(*O.quantize_tiles(w.float().numpy())), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_grouped_tiles_of_every_size_give_the_same_bits(device, dtype):
+    E, N, K = 9, 1281, 1500
+    counts = [700, 0, 1, 900, 129, 128, 3, 2000, 400]
+    off = np.concatenate([[0], np.cumsum(counts)])
+    x, w = rand((off[-1] + 200, K), dtype, 1, 0.3).to(device), rand((E, N, K), dtype, 2, 0.3).to(device)
+    h = Fp8Weight.quantize(w)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=device)
+    y = fp8_grouped_linear(x, h, ints(off))
+    assert (y[off[-1]:] == 0).all()
+    for e in range(E):
+        lo, hi = int(off[e]), int(off[e + 1])
+        part = x[lo:hi] if hi - lo > 64 else x[lo:lo + 65]  # (up to 64 rows take the fp16 sums)
+        one = ints([0] * (e + 1) + [hi - lo] * (E - e))
+        assert torch.equal(fp8_grouped_linear(part, h, one)[:hi - lo], y[lo:hi]), e
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("C", [512, 1024])
+def test_layers_of_every_size_give_the_same_bits(device, dtype, C):
+    """Sequences of a large batch and the same ones in a small batch."""
+    B, T, F, E, k = 40, 50, 1100, 8, 4
+    x = rand((B, T, C), dtype, 1, 0.5).to(device)
+    key, val = rand((E, F, C), dtype, 2, 0.05).to(device), rand((E, C, F), dtype, 3, 0.05).to(device)
+    x_k = rand((E, C), dtype, 4, 0.5).to(device)
+    gen = torch.Generator().manual_seed(5)
+    inds = torch.rand(B, T, E, generator=gen).argsort(-1)[..., :k].to(torch.int32).to(device)
+    gates = torch.rand(B, T, k, generator=gen).to(device)
+    hk, hv = Fp8Weight.quantize(key), Fp8Weight.quantize(val)
+    y = fp8_experts(x, inds, gates, x_k, hk, hv)
+    # (hidden values of some 1e4 times values: part of the fp16 results lie past 65504)
+    assert not y.isnan().any() and (dtype == "f16" or torch.isfinite(y).all())
+    for b in (0, 17, 37):
+        part = slice(b, b + 3)
+        got = fp8_experts(x[part].contiguous(), inds[part].contiguous(), gates[part].contiguous(), x_k, hk, hv)
+        assert torch.equal(got, y[part]), b
