@@ -381,17 +381,13 @@ class Fp8MoE_CMix(nn.Module):
                    Fp8Weight.quantize(layer.expert_key), Fp8Weight.quantize(layer.expert_val))
 
     def _apply(self, fn, recurse=True):
-        # a cast (.half(), .to(dtype)) is for the router and x_k: the weights go through it as integers
-        views = {f"{n}_q": torch.uint8 for n in ("key", "value")}
-        views.update({f"{n}_scale": torch.int32 for n in ("key", "value")})
-        was = {n: self._buffers[n].dtype for n in views}
-        for n, dt in views.items():
-            self._buffers[n] = self._buffers[n].view(dt)
-        try:
-            return super()._apply(fn, recurse)
-        finally:
-            for n, dt in was.items():
-                self._buffers[n] = self._buffers[n].view(dt)
+        # a cast (.half(), .to(dtype), .type(dtype)) is for the router and x_k: the weights move, as they are
+        was = {n: self._buffers[n] for n in ("key_q", "key_scale", "value_q", "value_scale")}
+        super()._apply(fn, recurse)
+        for n, t in was.items():
+            if self._buffers[n].dtype != t.dtype:
+                self._buffers[n] = t.to(self._buffers[n].device)
+        return self
 
     def forward(self, x: torch.Tensor, x_prev: torch.Tensor | None = None, residual: torch.Tensor | None = None):
         """(out, aux_loss, z_loss), as MoE_CMix's forward."""

@@ -113,7 +113,8 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None = 
 class GroupRouter(nn.Module):
     """A router of many experts: gate.weight (E, C), ``route_topk``'s options,
     and a bias that balances the experts' load without a loss
-    (``balance_bias``, a buffer: it ranks, it is not trained).
+    (``balance_bias``, a buffer: it ranks, it is not trained, and it stays
+    float32 when the module is cast, as small steps add up in it).
 
     Returns what ``Router`` returns, (inds (B,T,k) int32, weights (B,T,k) in
     x's dtype, aux_loss, z_loss), both losses 0: ``update_balance`` takes their
@@ -129,6 +130,13 @@ class GroupRouter(nn.Module):
         self.options = dict(score=score, n_groups=n_groups, top_groups=top_groups, group_score=group_score,
                             renormalize=renormalize, scale=scale)
         self.register_buffer("balance_bias", torch.zeros(n_experts))
+
+    def _apply(self, fn, recurse=True):
+        bias = self.balance_bias
+        super()._apply(fn, recurse)
+        if self.balance_bias.dtype != bias.dtype:  # a cast goes past the bias, a move does not
+            self.balance_bias = bias.to(self.balance_bias.device)
+        return self
 
     def forward(self, x: torch.Tensor):
         require_device(x, "GroupRouter")

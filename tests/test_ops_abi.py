@@ -7,8 +7,8 @@ import ctypes
 import pytest
 import torch
 
-from rwkv_mlx_amd import (Fp8Weight, _lib as L, fp8_experts, fp8_grouped_linear, fp8_linear, fp8_quantize,
-                          route_topk)
+from rwkv_mlx_amd import (Fp8MoE_CMix, Fp8Weight, GroupRouter, _lib as L, fp8_experts, fp8_grouped_linear, fp8_linear,
+                          fp8_quantize, route_topk)
 
 FAKE = 1 << 40
 
@@ -175,3 +175,23 @@ def test_launches_stay_below_2_to_32_threads():
     e.seq_len = (1 << 22) - 64
     e.d_model = 4096
     assert lib.rwkvmoe_fp8_experts_workspace_bytes(ref(e), ref(b)) == 0
+
+
+def test_casts_leave_the_balance_bias_and_8_bit_weights_alone():
+    """The bias adds up small steps: in bfloat16 1 + 0.001 is 1 again."""
+    r = GroupRouter(8, 16, 2)
+    r.balance_bias.fill_(1.0)
+    for cast in (lambda m: m.bfloat16(), lambda m: m.to(torch.float16), lambda m: m.type(torch.float64)):
+        assert cast(r) is r and r.balance_bias.dtype == torch.float32 and r.gate.weight.dtype != torch.float32
+        before = r.balance_bias.clone()
+        r.update_balance(torch.zeros(4, 2, dtype=torch.int32), rate=1e-3)
+        assert r.balance_bias[0] < before[0] and (r.balance_bias[1:] > before[1:]).all()
+    e4m3 = lambda *s: torch.arange(16 * 128, dtype=torch.float32).remainder(100).view(1, 16, 128).to(
+        torch.float8_e4m3fn)
+    w = Fp8Weight((1, 16, 128), e4m3(), torch.full((1, 1, 1), 0.3))
+    v = Fp8Weight((1, 128, 16), torch.zeros(1, 128, 128, dtype=torch.float8_e4m3fn), torch.ones(1, 1, 1))
+    m = Fp8MoE_CMix(r, torch.zeros(1, 128), w, v)
+    for cast in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.type(torch.float64)):
+        assert cast(m) is m and m.key_q.dtype == torch.float8_e4m3fn and m.key_scale.dtype == torch.float32
+        assert torch.equal(m.key_q.view(torch.uint8), w.q.view(torch.uint8)) and m.key_scale.item() == w.scale.item()
+        assert m.x_k.dtype != torch.float32
