@@ -17,6 +17,7 @@ block NaN.  Products are summed in fp32 and rounded once.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 from torch import nn
@@ -169,15 +170,6 @@ def _product(x, N, K, groups, code, q, scale, offsets, dtype):
     return out
 
 
-def _matmul(aq, a_s, bq, b_s, M, N, K, block, dtype, like):
-    """The product of two matrices in 8 bits, (M, K) and (N, K)."""
-    out = torch.empty(M, N, dtype=dtype, device=aq.device)
-    desc = _lib.fp8_desc(M, N, K, 0, _lib.TORCH_DTYPE_CODE[dtype], block, K)
-    _call("rwkvmoe_fp8_matmul", like, desc, aq.data_ptr(), a_s.data_ptr(), bq.data_ptr(),
-          b_s.data_ptr(), None, out.data_ptr())
-    return out
-
-
 class _FrozenFunction(torch.autograd.Function):
     """x · wᵀ with a frozen weight; d x = d y · w, d y rounded like x."""
 
@@ -200,6 +192,34 @@ class _FrozenFunction(torch.autograd.Function):
                         ctx.dtype), None, None
 
 
+@lru_cache(maxsize=1024)
+def _parts(*wanted):
+    """(offsets, bytes) of 8-bit matrices in one allocation: for each (rows,
+    columns, scales) its values and its scales, for None neither."""
+    at, out = 0, []
+    for part in wanted:
+        if part is None:
+            out += [None, None]
+            continue
+        rows, cols, scales = part
+        for n in (rows * _blocks(cols) * BLOCK, scales * 4):
+            out.append(at)
+            at += -(-n // 256) * 256
+    return out, at
+
+
+def _alloc(device, *wanted):
+    """One allocation for the matrices of ``_parts``, and their addresses."""
+    offsets, n = _parts(*wanted)
+    buf = torch.empty(n, dtype=torch.uint8, device=device)
+    return buf, _at(buf, offsets)
+
+
+def _at(buf: torch.Tensor, offsets):
+    base = buf.data_ptr()
+    return [None if o is None else base + o for o in offsets]
+
+
 class _LinearFunction(torch.autograd.Function):
     """x · wᵀ with a trainable weight, all three products in 8 bits:
     y = x · wᵀ, d x = d y · w, d w = d yᵀ · x (both rounded in blocks along the
@@ -210,27 +230,43 @@ class _LinearFunction(torch.autograd.Function):
         R, K = x.shape
         N = w.shape[0]
         need_x, need_w = ctx.needs_input_grad
-        wq = Fp8Weight.quantize(w, transposed=need_x)
-        if need_w:
-            xq, xs, xqt, xst = fp8_quantize(x, transposed=True)
-        else:
-            (xq, xs), xqt, xst = fp8_quantize(x), None, None
-        ctx.save_for_backward(xqt, xst, wq.q_t, wq.scale_t)
-        ctx.sizes = (R, N, K, x.dtype, w.dtype)
-        return _matmul(xq, xs, wq.q, wq.scale, R, N, K, _lib.FP8_TILES, x.dtype, x)
+        Rb, Nb, Kb = _blocks(R), _blocks(N), _blocks(K)
+        dev, xc, wc = x.device, _lib.TORCH_DTYPE_CODE[x.dtype], _lib.TORCH_DTYPE_CODE[w.dtype]
+        w = w.contiguous()
+        keep = ((K, N, Kb * Nb) if need_x else None, (K, R, Rb * K) if need_w else None)
+        kept, back = _alloc(dev, *keep)
+        tmp, ahead = _alloc(dev, (N, K, Nb * Kb), (R, K, Kb * R))
+        _call("rwkvmoe_fp8_quantize", w, _lib.fp8_desc(N, 0, K, 0, wc, _lib.FP8_TILES, K), w.data_ptr(), *ahead[:2],
+              *back[:2])
+        _call("rwkvmoe_fp8_quantize", x, _lib.fp8_desc(R, 0, K, 0, xc, _lib.FP8_ROWS, _stride(x)), x.data_ptr(),
+              *ahead[2:], *back[2:])
+        y = torch.empty(R, N, dtype=x.dtype, device=dev)
+        _call("rwkvmoe_fp8_matmul", x, _lib.fp8_desc(R, N, K, 0, xc, _lib.FP8_TILES, K), *ahead[2:], *ahead[:2], None,
+              y.data_ptr())
+        ctx.save_for_backward(kept)
+        ctx.plan = (R, N, K, x.dtype, w.dtype, keep)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xqt, xst, wqt, wst = ctx.saved_tensors
-        R, N, K, xdt, wdt = ctx.sizes
+        R, N, K, xdt, wdt, keep = ctx.plan
+        (kept,) = ctx.saved_tensors
+        back = _at(kept, _parts(*keep)[0])
         need_x, need_w = ctx.needs_input_grad
-        parts = fp8_quantize(_rows2d(dy), transposed=need_w, rows=need_x)
+        dy, dev = _rows2d(dy), dy.device
+        tmp, g = _alloc(dev, (R, N, _blocks(N) * R) if need_x else None, (N, R, _blocks(R) * N) if need_w else None)
+        _call("rwkvmoe_fp8_quantize", dy, _lib.fp8_desc(R, 0, N, 0, _code(dy, "fp8_linear"), _lib.FP8_ROWS, _stride(dy)),
+              dy.data_ptr(), *g)
         dx = dw = None
         if need_x:
-            dx = _matmul(*parts[:2], wqt, wst, R, K, N, _lib.FP8_TILES, xdt, dy)
+            dx = torch.empty(R, K, dtype=xdt, device=dev)
+            _call("rwkvmoe_fp8_matmul", dy, _lib.fp8_desc(R, K, N, 0, _lib.TORCH_DTYPE_CODE[xdt], _lib.FP8_TILES, N),
+                  *g[:2], *back[:2], None, dx.data_ptr())
         if need_w:
-            dw = _matmul(*parts[-2:], xqt, xst, N, K, R, _lib.FP8_ROWS, wdt, dy)
+            dw = torch.empty(N, K, dtype=wdt, device=dev)
+            _call("rwkvmoe_fp8_matmul", dy, _lib.fp8_desc(N, K, R, 0, _lib.TORCH_DTYPE_CODE[wdt], _lib.FP8_ROWS, R),
+                  *g[2:], *back[2:], None, dw.data_ptr())
         return dx, dw
 
 
@@ -272,6 +308,8 @@ def fp8_linear(x: torch.Tensor, weight) -> torch.Tensor:
             y = _product(x2, N, K, 0, _lib.TORCH_DTYPE_CODE[x2.dtype], weight.q, weight.scale, None, x2.dtype)
     else:
         _code(weight, "fp8_linear")
+        if min(weight.shape) < 1:
+            raise ValueError(f"fp8_linear: a weight (N, K) expected, got {tuple(weight.shape)}")
         if grad and (x.requires_grad or weight.requires_grad):
             y = _LinearFunction.apply(x2, weight)
         else:

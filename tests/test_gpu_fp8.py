@@ -516,3 +516,23 @@ def test_layers_of_every_size_give_the_same_bits(device, dtype, C):
         part = slice(b, b + 3)
         got = fp8_experts(x[part].contiguous(), inds[part].contiguous(), gates[part].contiguous(), x_k, hk, hv)
         assert torch.equal(got, y[part]), b
+
+
+def test_what_the_backward_keeps(device):
+    """The operands kept for a linear's backward can be kept elsewhere (saved
+    tensor hooks), read twice, and are gone after the last backward."""
+    x = rand((150, 256), "bf16", 1).to(device).requires_grad_(True)
+    w = rand((200, 256), "f32", 2).to(device).requires_grad_(True)
+    dy = rand((150, 200), "bf16", 4).to(device)
+    y = fp8_linear(x, w)
+    want = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, w), dy), want))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, (x, w), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = fp8_linear(x, w)
+    filler = torch.full((1 << 20,), 255, dtype=torch.uint8, device=device)  # (over what the call has freed)
+    got = torch.autograd.grad(y, (x, w), dy)
+    assert filler.min() == 255 and all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(torch.autograd.grad(fp8_linear(x, w.detach()), x, dy)[0], want[0])
+    assert torch.equal(torch.autograd.grad(fp8_linear(x.detach(), w), w, dy)[0], want[1])
