@@ -429,6 +429,8 @@ class Fp8MoE_CMix(nn.Module):
 
     def forward(self, x: torch.Tensor, x_prev: torch.Tensor | None = None, residual: torch.Tensor | None = None):
         """(out, aux_loss, z_loss), as MoE_CMix's forward."""
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, x_prev, residual)):
+            raise RuntimeError("Fp8MoE_CMix has no gradient: call it under torch.no_grad(), or train with MoE_CMix")
         with torch.no_grad():
             inds, gates, aux, z = self.router(x)
             key = Fp8Weight(self._shapes[0], self.key_q, self.key_scale)

@@ -140,7 +140,10 @@ class GroupRouter(nn.Module):
 
     def forward(self, x: torch.Tensor):
         require_device(x, "GroupRouter")
-        # fp32 logits: which expert is taken hangs on small differences
+        # fp32 logits, also under autocast: which expert is taken hangs on small differences
+        if torch.is_autocast_enabled("cuda"):
+            with torch.autocast("cuda", enabled=False):
+                return self.forward(x)
         logits = nn.functional.linear(x.to(torch.float32), self.gate.weight.to(torch.float32))
         inds, gates = route_topk(logits, self.top_k, bias=self.balance_bias, **self.options)
         zero = torch.zeros((), dtype=torch.float32, device=x.device)

@@ -536,3 +536,19 @@ def test_what_the_backward_keeps(device):
     assert filler.min() == 255 and all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(torch.autograd.grad(fp8_linear(x, w.detach()), x, dy)[0], want[0])
     assert torch.equal(torch.autograd.grad(fp8_linear(x.detach(), w), w, dy)[0], want[1])
+
+
+def test_the_layer_refuses_to_drop_a_gradient(device):
+    torch.manual_seed(3)
+    r = GroupRouter(64, 4, 2).to(device)
+    key, val = rand((4, 96, 64), "bf16", 1).to(device), rand((4, 64, 96), "bf16", 2).to(device)
+    m = Fp8MoE_CMix(r, torch.zeros(4, 64, device=device), Fp8Weight.quantize(key), Fp8Weight.quantize(val))
+    x = rand((2, 3, 64), "bf16", 3).to(device)
+    want = m(x)[0]
+    x.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        m(x)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        m(x.detach(), residual=x)
+    with torch.no_grad():
+        assert torch.equal(m(x)[0], want)

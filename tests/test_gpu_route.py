@@ -252,3 +252,18 @@ def test_route_gradient_in_a_graph(device):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, step())
+
+
+@pytest.mark.parametrize("score,want", [("sigmoid", 2), ("softmax", 5)])
+def test_group_router_keeps_fp32_logits_under_autocast(device, score, want):
+    """Two experts with logits of 64 and 64 (1 + 2^-12): bf16 logits tie and
+    leave expert 2 in front.  So do their sigmoids, 1 - e^-64 = 1 - 2^-92 in 64
+    bits, but not their softmax."""
+    r = GroupRouter(64, 8, 1, score=score).to(device)
+    with torch.no_grad():
+        r.gate.weight.zero_()
+        r.gate.weight[5], r.gate.weight[2] = 1.0 + 2.0 ** -12, 1.0
+    x = torch.ones(1, 3, 64, device=device)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        inds, w, _, _ = r(x)
+    assert (inds == want).all() and w.dtype == x.dtype and torch.equal(inds, r(x)[0])
