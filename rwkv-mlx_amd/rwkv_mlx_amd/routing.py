@@ -118,7 +118,8 @@ class GroupRouter(nn.Module):
 
     Returns what ``Router`` returns, (inds (B,T,k) int32, weights (B,T,k) in
     x's dtype, aux_loss, z_loss), both losses 0: ``update_balance`` takes their
-    place."""
+    place.  It routes for ``Fp8MoE_CMix`` and for layers that call their router;
+    the layers whose kernels route by themselves refuse it."""
 
     def __init__(self, d_model: int, n_experts: int, top_k: int = 2, score: str = "sigmoid", n_groups: int = 1,
                  top_groups: int | None = None, group_score: str = "top2", renormalize: bool = True,
@@ -130,6 +131,12 @@ class GroupRouter(nn.Module):
         self.options = dict(score=score, n_groups=n_groups, top_groups=top_groups, group_score=group_score,
                             renormalize=renormalize, scale=scale)
         self.register_buffer("balance_bias", torch.zeros(n_experts))
+
+    @property
+    def logit_bias(self):
+        # the fused layers read their router's weights, not its result
+        raise TypeError("this layer routes in its own kernels, by softmax and top-k; a GroupRouter goes with "
+                        "Fp8MoE_CMix")
 
     def _apply(self, fn, recurse=True):
         bias = self.balance_bias

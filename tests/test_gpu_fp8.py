@@ -552,3 +552,12 @@ def test_the_layer_refuses_to_drop_a_gradient(device):
         m(x.detach(), residual=x)
     with torch.no_grad():
         assert torch.equal(m(x)[0], want)
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_a_fused_layer_refuses_a_group_router(device, train):
+    layer = MoE_CMix(RWKVConfig(n_embd=64, dim_ffn=128), 0, 4, 2).to(device)
+    layer.router = GroupRouter(64, 4, 2).to(device)
+    x = torch.randn(1, 3, 64, device=device, requires_grad=train)
+    with torch.set_grad_enabled(train), pytest.raises(TypeError, match="GroupRouter"):
+        layer(x)

@@ -2,6 +2,7 @@
 call here reaches a launch."""
 from __future__ import annotations
 
+import copy
 import ctypes
 
 import pytest
@@ -195,3 +196,11 @@ def test_casts_leave_the_balance_bias_and_8_bit_weights_alone():
         assert cast(m) is m and m.key_q.dtype == torch.float8_e4m3fn and m.key_scale.dtype == torch.float32
         assert torch.equal(m.key_q.view(torch.uint8), w.q.view(torch.uint8)) and m.key_scale.item() == w.scale.item()
         assert m.x_k.dtype != torch.float32
+
+
+def test_fused_layers_refuse_a_group_router():
+    """Their kernels route by the router's weight alone, after they have read its logit_bias."""
+    r = GroupRouter(8, 4, 2)
+    with pytest.raises(TypeError, match="Fp8MoE_CMix"):
+        r.logit_bias
+    assert set(r.state_dict()) == {"gate.weight", "balance_bias"} and copy.deepcopy(r).top_k == 2
