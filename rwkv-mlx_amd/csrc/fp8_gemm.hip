@@ -874,10 +874,13 @@ hipError_t run_tiles(const Fp8Gemm& p, hipStream_t s) {
   // 117, 105; 8192 x 8192 x 1024 94, 101; 4096 x 1024 x 4096 (96 wide tiles) 27, 44.
   // Hidden rows are half the bytes of 16-bit results, so their epilogue pays for
   // itself sooner: 32496 rows of 32 experts x 4096 x 1024 285, 249.
-  // Where 128 x 128 tiles leave half of the CUs idle, 64 x 128 ones read more
-  // but are sooner done (us, 128 x 128 against 64 x 128): 200 x 4096 x 1024 9.4,
-  // 8.1; 1024 x 2048 x 1024 9.4, 8.6; with more tiles 2048 x 2048 x 1024 10.4,
-  // 11.6; 300 x 8192 x 8192 45.8, 51.8.
+  // Where 128 x 128 tiles leave half of the CUs idle, or are a quarter more than
+  // there are CUs at most, so that few CUs take two, 64 x 128 ones read more but
+  // are sooner done (us, 128 x 128 against 64 x 128; in brackets the tiles a CU):
+  // 200 x 4096 x 1024 (1/4) 9.4, 8.1; 1024 x 2048 x 1024 (1/2) 9.4, 8.6;
+  // 300 x 8192 x 8192 (3/4) 45.8, 51.8; 2048 x 2048 x 1024 (1) 10.4, 11.6;
+  // 300 x 12288 x 2048 (1.1) 20.9, 18.3; 2560 x 2048 x 4096 (1.25) 37.7, 36.4;
+  // 2048 x 3584 x 1024 (1.75) 15.1, 17.8.
   if constexpr (BKIND == FP8_TILES) {
     const long long cus = num_cus();
     auto tiles = [&](int bm, int bn) {
@@ -888,7 +891,9 @@ hipError_t run_tiles(const Fp8Gemm& p, hipStream_t s) {
       if (p.k > (OUT == FP8_OUT_RELU2Q ? 7 : 11) * 128 && wide * 5 >= (wide + cus - 1) / cus * cus * 4)
         return run_tile<192, 256, 2, 2, 1, 3, BKIND, OUT, GRP, EX>(p, s);
     }
-    if (tiles(128, 128) * 2 <= cus) return run_tile<64, 128, 2, 1, 3, 2, BKIND, OUT, GRP, EX>(p, s);
+    const long long t = tiles(128, 128);
+    if (t * 2 <= cus || (t > cus && t * 4 <= cus * 5))
+      return run_tile<64, 128, 2, 1, 3, 2, BKIND, OUT, GRP, EX>(p, s);
   }
   return run_tile<128, 128, 4, 1, 2, 2, BKIND, OUT, GRP, EX>(p, s);
 }

@@ -467,13 +467,13 @@ def test_gradients_in_a_graph(device):
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("N,K", [(2690, 1500), (2688, 1500), (2691, 300)])
 def test_tiles_of_every_size_give_the_same_bits(device, dtype, N, K):
-    """A row's sums take one order whatever tile holds it: 64 x 128 with 300
-    rows, 128 x 128 with 1500, 192 x 256 with 3840 (16-bit results, K > 11
-    blocks), and the first of these is held against the formula."""
+    """A row's sums take one order whatever tile holds it: 64 x 128 with 300 and
+    1500 rows, 128 x 128 with 900, 192 x 256 with 3840 (16-bit results, K > 11
+    blocks), and the last of these is held against the formula."""
     x, w = rand((3840, K), dtype, 1, 0.3), rand((N, K), dtype, 2, 0.3)
     h, xd = Fp8Weight.quantize(w.to(device)), x.to(device)
     all_rows = fp8_linear(xd, h)
-    for r in (65, 300, 1500):
+    for r in (65, 300, 900, 1500):
         assert torch.equal(fp8_linear(xd[:r], h), all_rows[:r]), r
     assert torch.equal(fp8_linear(xd[3000:], h), all_rows[3000:])
     close(all_rows[:100], O.held_rows(*O.quantize_rows(x[:100].float().numpy())),
